@@ -23,7 +23,7 @@ LIB_PATH = os.path.join(HERE, "libacfun_b200.so")
 _lock = threading.Lock()
 _lib = None
 
-vp, i, f, sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+vp, i, f, sz, ll = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_longlong
 
 # every exported entry point with its ctypes signature (restype, argtypes)
 SIGNATURES = {
@@ -60,6 +60,11 @@ SIGNATURES = {
     "acfun_gemm_s8_requant": (None, [i, i, i, vp, vp, vp, vp, vp, i]),
     "acfun_gemm_epi_noalloc": (i, [i, i, i, vp, vp, vp, vp, i]),
     "acfun_set_fp32_math": (i, [i]),
+    "acfun_rope_frequencies": (i, [i, C.c_double, i, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp]),
+    "acfun_rope": (i, [vp, vp, i, i, i, i, ll, ll, ll, ll, vp, vp]),
+    "acfun_kv8_append": (i, [vp, vp, vp, vp, i, ll, ll, ll, ll, vp]),
+    "acfun_kv8_read": (i, [vp, vp, vp, vp, i]),
+    "acfun_kv8_attention": (i, [vp, vp, vp, vp, i, i, ll, ll, ll, ll, f, i, i, vp]),
     "acfun_set_stream": (None, [vp]),
     "acfun_get_stream": (vp, []),
     "acfun_set_device": (i, [i]),
@@ -322,3 +327,7 @@ class Model:
             self.close()
         except Exception:
             pass
+
+
+# ------------------------------------------------------------------ attention over an int8 cache
+from .kv8 import KvBatch, KvCache8, Rope, rope, rope_frequencies  # noqa: E402,F401

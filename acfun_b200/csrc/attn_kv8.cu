@@ -1,0 +1,521 @@
+// attn_kv8.cu — attention over the int8 cache (acfun_kv8_attention): the entry point and the
+// streaming kernel, which reads codes straight from global memory into matrix-instruction
+// fragments.  It takes any shape; attention with few rows per cache head (decode steps, drafts)
+// is bound by the codes it reads, and that is what it is built for.
+//
+// Rows: the new tokens of a sequence times the query heads that share a cache head, row = token *
+// group + head, in tiles of 16.  A block of four warps takes one (sequence, cache head, row tile,
+// chunk of keys); its warps take units of 16 keys in turn, each with its own running maximum, sum
+// and output, which are joined in shared memory at the end.  A long sequence is split over
+// blocks; the last of them to finish joins their parts in the order of the chunks, so the result
+// does not depend on who was last.
+//
+// Mathematics.  With q scaled per row by a power of two to fp16 range (exact for what matters:
+// 11 bits below the row's largest element), codes c exact in fp16, S = q.c_k in fp32,
+//   t = S * (scale * s_k[page]) log2 e + log2 s_v[page],  w = 2^(t - m) in fp16,  O += w c_v,
+//   l += (sum of w over the page's keys, in fp32 before rounding) / s_v[page],  out = O / l.
+// The V scale rides in the exponent, so O needs no per-page scaling and w stays within fp16 range
+// whatever the scales are; m moves only when a weight would pass 2^15.
+//
+// Fragments.  K is the B operand of m16n8k16 with its contraction index (the element of a head)
+// permuted so that a thread's share of a key is 16 consecutive bytes; V is the B operand with its
+// column index permuted so that a thread's share of each of its four keys is 16 consecutive bytes
+// (8 when dim is 64).  Both come by 16-byte loads, whole sectors, with no staging.
+#include <math.h>
+
+#include <algorithm>
+
+#include "attn.cuh"
+
+namespace acf {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kUnit = 16;          // keys per step of a warp
+constexpr int kMaxPages = 1024;    // pages of one chunk (their scales are staged in shared memory)
+// Weights are kept within fp16's upper range, so that keys far below the largest keep their bits:
+// a row's offset m is set so that its largest weight is 2^kTop, and moves when one would pass
+// 2^kMost.
+constexpr float kTop = 7.0f, kMost = 15.0f;
+constexpr int kTickets = 1 << 16;
+
+struct StreamArgs {
+  AttnArgs a;
+  int chunk;                 // keys per block, a multiple of kUnit
+  int splits;                // chunks of max_len keys (the stride of the partial results)
+  float* part_o;             // [tokens][q_heads][splits][DIM], null when splits == 1
+  float2* part_ml;           // [tokens][q_heads][splits]
+  unsigned* tickets;         // [seqs][heads][row tiles], zero between calls
+  int row_tiles;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 1);
+  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+}
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+
+// What a page needs in the loop: its place, and its scales in the forms used.
+struct PageEntry {
+  int pid;          // -1: out of range (reported), its keys are not seen
+  float ks;         // scale * k scale * log2 e
+  float lv, rv;     // log2 and reciprocal of the v scale
+};
+
+template <typename T>
+__device__ __forceinline__ void store2(T* p, float a, float b) {
+  p[0] = from_f<T>(a);
+  p[1] = from_f<T>(b);
+}
+
+template <int DIM>
+struct StreamSmem {
+  PageEntry pages[kMaxPages];
+  float2 ml[kWarps][16];
+  float row_ml[16][2];
+  int last;
+  float o[kWarps][16][DIM + 4];
+};
+
+// DIM / 64 runs of 16 bytes per key for K; DIM / 8 bytes per key for V.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p, unsigned* err) {
+  constexpr int KR = DIM / 64;          // 16-byte runs of a thread per key (K)
+  constexpr int NT = DIM / 8;           // output n-tiles
+  constexpr int VW = DIM / 32;          // 32-bit words of a thread per key (V)
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  StreamSmem<DIM>& sm = *reinterpret_cast<StreamSmem<DIM>*>(smem_raw);
+  const AttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int head = blockIdx.x % a.kv.heads, rt = blockIdx.x / a.kv.heads, seq = blockIdx.y, chunk_i = blockIdx.z;
+  const SeqView sv = seq_view(a.b, seq, err);
+  const int rows = sv.n * a.group;
+  const int r0 = rt * 16;
+  if (r0 >= rows) return;
+  const int nr = min(16, rows - r0);
+  const int t_first = r0 / a.group, t_last = (r0 + nr - 1) / a.group;
+  const int pos0 = sv.len - sv.n;  // position of new token 0 (negative: it sees nothing)
+  const int key_hi = a.causal ? max(0, min(sv.len, pos0 + t_last + 1)) : sv.len;
+  const int key_lo = a.window > 0 ? max(0, pos0 + t_first - a.window + 1) : 0;
+  const int unit0 = key_lo / kUnit, units = key_hi > key_lo ? (key_hi + kUnit - 1) / kUnit - unit0 : 0;
+  const int per = p.chunk / kUnit;
+  const int nsplit = max(1, (units + per - 1) / per);
+  if (chunk_i >= nsplit) return;
+  const int ub = unit0 + chunk_i * per, ue = min(unit0 + units, ub + per);
+
+  // the chunk's pages
+  const int lg = a.kv.page_log2;
+  const int pg0 = (ub * kUnit) >> lg;
+  const int npg = ue > ub ? (((ue * kUnit - 1) >> lg) - pg0 + 1) : 0;
+  for (int i = threadIdx.x; i < npg; i += blockDim.x) {
+    PageEntry e = {-1, 0.0f, 0.0f, 0.0f};
+    e.pid = seq_page(a.b, seq, pg0 + i, a.kv.pages, err);
+    if (e.pid >= 0) {
+      const size_t sc = (size_t)e.pid * a.kv.heads + head;
+      const float vs = fmaxf(a.kv.vs[sc], 0x1p-100f);
+      e.ks = a.scale * a.kv.ks[sc] * 1.4426950408889634f;
+      e.lv = log2f(vs);
+      e.rv = 1.0f / vs;
+    }
+    sm.pages[i] = e;
+  }
+
+  // Q fragments of rows g and g + 8, scaled by a power of two per row
+  uint32_t qf[DIM / 16][4];
+  float q_unit[2];
+  {
+    const T* q = static_cast<const T*>(a.q);
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+      const int r = r0 + g + 8 * rr;
+      const bool in = g + 8 * rr < nr;
+      const int t = r / a.group, hq = head * a.group + r - t * a.group;
+      const T* src = q + (long long)(sv.row0 + t) * a.q_token + (long long)hq * a.q_head;
+      float top = 0.0f;
+      // two passes over the row (the second is in cache): the largest element, then the values
+      if (in) {
+        for (int i = 0; i < DIM / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to_f(src[(i / 4) * 64 + c * 16 + 4 * (i % 4) + e])));
+      }
+      top = quad_max(top);
+      int ex = 0;
+      if (top > 0.0f && top <= 3.4028234663852886e38f) frexpf(top, &ex);
+      ex = min(max(ex, -100), 126);
+      const float down = exp2f((float)-ex);
+      q_unit[rr] = exp2f((float)ex);
+#pragma unroll
+      for (int i = 0; i < DIM / 16; ++i) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[e] = in ? to_f(src[(i / 4) * 64 + c * 16 + 4 * (i % 4) + e]) * down : 0.0f;
+        qf[i][rr] = pack_f16(x[0], x[1]);
+        qf[i][2 + rr] = pack_f16(x[2], x[3]);
+      }
+    }
+  }
+  // the keys rows g and g + 8 see: [lo, hi)
+  int see_lo[2], see_hi[2];
+#pragma unroll
+  for (int rr = 0; rr < 2; ++rr) {
+    const int pos = pos0 + (r0 + g + 8 * rr) / a.group;
+    see_hi[rr] = a.causal ? min(sv.len, pos + 1) : sv.len;
+    see_lo[rr] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    if (pos < 0) see_hi[rr] = 0;
+  }
+  // units that every row of the tile sees whole
+  const int all_lo = a.window > 0 ? max(0, pos0 + t_last - a.window + 1) : 0;
+  const int all_hi = pos0 + t_first < 0 ? 0 : a.causal ? min(sv.len, pos0 + t_first + 1) : sv.len;
+
+  float o[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  __syncthreads();
+
+  uint4 kr[2][KR];
+  uint32_t vr[4][VW];
+  auto place = [&](int u) -> size_t {  // byte offset of the unit's first key, this head
+    const PageEntry& e = sm.pages[((u * kUnit) >> lg) - pg0];
+    const int slot = (u * kUnit) & (a.kv.page - 1);
+    return (((size_t)max(e.pid, 0) * a.kv.heads + head) * a.kv.page + slot) * DIM;
+  };
+  auto load_k = [&](int u) {
+    const int8_t* b = a.kv.k + place(u) + g * DIM + c * 16;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < KR; ++r) kr[t][r] = ldg16(b + t * 8 * DIM + r * 64);
+  };
+  auto load_v = [&](int u) {
+    const int8_t* b = a.kv.v + place(u) + g * (DIM / 8);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int8_t* s = b + (2 * c + (k & 1) + 8 * (k >> 1)) * DIM;
+      if constexpr (DIM == 64) {
+        const uint2 w = ldg8(s);
+        vr[k][0] = w.x, vr[k][1] = w.y;
+      } else {
+#pragma unroll
+        for (int r = 0; r < VW / 4; ++r) {
+          const uint4 w = ldg16(s + 16 * r);
+          vr[k][4 * r] = w.x, vr[k][4 * r + 1] = w.y, vr[k][4 * r + 2] = w.z, vr[k][4 * r + 3] = w.w;
+        }
+      }
+    }
+  };
+
+  int u = ub + warp;
+  if (u < ue) {
+    load_k(u);
+    load_v(u);
+  }
+  for (; u < ue; u += kWarps) {
+    const PageEntry e = sm.pages[((u * kUnit) >> lg) - pg0];
+    // S: two n-tiles of 8 keys
+    float s[2][4] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < KR; ++r) {
+        const uint32_t w[4] = {kr[t][r].x, kr[t][r].y, kr[t][r].z, kr[t][r].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = w[i] ^ 0x80808080u;
+          const int ks = r * 4 + i;
+          mma_f16(s[t], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], f16_from_u8(x, 0x4140), f16_from_u8(x, 0x4342));
+        }
+      }
+    const bool more = u + kWarps < ue;
+    if (more) load_k(u + kWarps);
+    // scores in powers of two, masked where the unit crosses an edge of what some row sees
+    const int k0 = u * kUnit;
+    const float f0 = e.ks * q_unit[0], f1 = e.ks * q_unit[1];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t][0] = fmaf(s[t][0], f0, e.lv), s[t][1] = fmaf(s[t][1], f0, e.lv);
+      s[t][2] = fmaf(s[t][2], f1, e.lv), s[t][3] = fmaf(s[t][3], f1, e.lv);
+    }
+    if (k0 < all_lo || k0 + kUnit > all_hi || e.pid < 0) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 8 * t + 2 * c + (i & 1);
+          if (key < see_lo[i >> 1] || key >= see_hi[i >> 1] || e.pid < 0) s[t][i] = -INFINITY;
+        }
+    }
+    const float top0 = quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])));
+    const float top1 = quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])));
+    if (__any_sync(0xffffffffu, top0 > m[0] + kMost || top1 > m[1] + kMost)) {
+      const float n0 = fmaxf(m[0], top0 - kTop), n1 = fmaxf(m[1], top1 - kTop);
+      const float b0 = m[0] == n0 ? 1.0f : exp2f(m[0] - n0), b1 = m[1] == n1 ? 1.0f : exp2f(m[1] - n1);
+      m[0] = n0, m[1] = n1;
+      l[0] *= b0, l[1] *= b1;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[i][0] *= b0, o[i][1] *= b0, o[i][2] *= b1, o[i][3] *= b1;
+    }
+    // a row that has seen nothing yet has m = -inf and only -inf scores
+    const float m0 = m[0] == -INFINITY ? 0.0f : m[0], m1 = m[1] == -INFINITY ? 0.0f : m[1];
+    float w[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      w[t][0] = exp2f(s[t][0] - m0), w[t][1] = exp2f(s[t][1] - m0);
+      w[t][2] = exp2f(s[t][2] - m1), w[t][3] = exp2f(s[t][3] - m1);
+    }
+    l[0] = fmaf((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]), e.rv, l[0]);
+    l[1] = fmaf((w[0][2] + w[0][3]) + (w[1][2] + w[1][3]), e.rv, l[1]);
+    const uint32_t a0 = pack_f16(w[0][0], w[0][1]), a1 = pack_f16(w[0][2], w[0][3]);
+    const uint32_t a2 = pack_f16(w[1][0], w[1][1]), a3 = pack_f16(w[1][2], w[1][3]);
+    // O: n-tile j holds elements (lane / 4) * DIM / 8 + j of the head
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+      const uint32_t x0 = vr[0][i] ^ 0x80808080u, x1 = vr[1][i] ^ 0x80808080u;
+      const uint32_t x2 = vr[2][i] ^ 0x80808080u, x3 = vr[3][i] ^ 0x80808080u;
+      const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
+      const uint32_t s0 = __byte_perm(x2, x3, 0x5140), s1 = __byte_perm(x2, x3, 0x7362);
+      mma_f16(o[4 * i], a0, a1, a2, a3, f16_from_u8(p0, 0x4140), f16_from_u8(s0, 0x4140));
+      mma_f16(o[4 * i + 1], a0, a1, a2, a3, f16_from_u8(p0, 0x4342), f16_from_u8(s0, 0x4342));
+      mma_f16(o[4 * i + 2], a0, a1, a2, a3, f16_from_u8(p1, 0x4140), f16_from_u8(s1, 0x4140));
+      mma_f16(o[4 * i + 3], a0, a1, a2, a3, f16_from_u8(p1, 0x4342), f16_from_u8(s1, 0x4342));
+    }
+    if (more) load_v(u + kWarps);
+  }
+
+  // ---- the four warps' parts joined
+  l[0] = quad_sum(l[0]), l[1] = quad_sum(l[1]);
+  if (c == 0) {
+    sm.ml[warp][g] = make_float2(m[0], l[0]);
+    sm.ml[warp][g + 8] = make_float2(m[1], l[1]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rr = 0; rr < 2; ++rr) {
+    const int r = g + 8 * rr;
+    float top = -INFINITY;
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.ml[w][r].x);
+    const float b = m[rr] == top ? 1.0f : exp2f(m[rr] - top);
+    if (r < nr) {
+      // thread's columns 2c, 2c + 1 of n-tile j are elements (2c) * NT + j and (2c + 1) * NT + j
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        sm.o[warp][r][2 * c * NT + j] = o[j][2 * rr] * b;
+        sm.o[warp][r][(2 * c + 1) * NT + j] = o[j][2 * rr + 1] * b;
+      }
+    }
+    if (warp == 0 && c == 0) {
+      float sum = 0.0f;
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 x = sm.ml[w][r];
+        sum += x.x == top ? x.y : x.y * exp2f(x.x - top);
+      }
+      sm.row_ml[r][0] = top, sm.row_ml[r][1] = sum;
+    }
+  }
+  __syncthreads();
+  T* out = static_cast<T*>(a.out);
+  for (int i = threadIdx.x; i < nr * (DIM / 2); i += blockDim.x) {
+    const int r = i / (DIM / 2), d = 2 * (i % (DIM / 2));
+    float x = 0.0f, y = 0.0f;
+    for (int w = 0; w < kWarps; ++w) x += sm.o[w][r][d], y += sm.o[w][r][d + 1];
+    const int t = (r0 + r) / a.group, hq = head * a.group + (r0 + r) - t * a.group;
+    const float top = sm.row_ml[r][0], sum = sm.row_ml[r][1];
+    if (nsplit == 1) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      store2(out + (long long)(sv.row0 + t) * a.o_token + (long long)hq * a.o_head + d, x * inv, y * inv);
+      if (d == 0 && a.lse)
+        a.lse[(long long)(sv.row0 + t) * a.q_heads + hq] =
+            sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+    } else {
+      const size_t at = ((size_t)(sv.row0 + t) * a.q_heads + hq) * p.splits + chunk_i;
+      *reinterpret_cast<float2*>(p.part_o + at * DIM + d) = make_float2(x, y);
+      if (d == 0) p.part_ml[at] = make_float2(top, sum);
+    }
+  }
+  if (nsplit == 1) return;
+
+  // ---- the last block of this row tile joins the chunks
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned* ticket = p.tickets + ((size_t)seq * a.kv.heads + head) * p.row_tiles + rt;
+    const unsigned before = atomicAdd(ticket, 1u);
+    sm.last = before == (unsigned)nsplit - 1;
+    if (sm.last) *ticket = 0;
+  }
+  __syncthreads();
+  if (!sm.last) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < nr * (DIM / 2); i += blockDim.x) {
+    const int r = i / (DIM / 2), d = 2 * (i % (DIM / 2));
+    const int t = (r0 + r) / a.group, hq = head * a.group + (r0 + r) - t * a.group;
+    const size_t at = ((size_t)(sv.row0 + t) * a.q_heads + hq) * p.splits;
+    float top = -INFINITY, x = 0.0f, y = 0.0f, sum = 0.0f;
+    for (int k = 0; k < nsplit; ++k) top = fmaxf(top, __ldcg(&p.part_ml[at + k]).x);
+    for (int k = 0; k < nsplit; ++k) {
+      const float2 ml = __ldcg(&p.part_ml[at + k]);
+      const float b = ml.x == top ? 1.0f : exp2f(ml.x - top);
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(p.part_o + (at + k) * DIM + d));
+      sum = fmaf(ml.y, b, sum), x = fmaf(v.x, b, x), y = fmaf(v.y, b, y);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    store2(out + (long long)(sv.row0 + t) * a.o_token + (long long)hq * a.o_head + d, x * inv, y * inv);
+    if (d == 0 && a.lse)
+      a.lse[(long long)(sv.row0 + t) * a.q_heads + hq] =
+          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+  }
+}
+
+// Zeroed once per device; the kernel leaves it zero.
+unsigned* tickets_of(int device) {
+  static unsigned* buf[64] = {};
+  if (device < 0 || device >= 64) return nullptr;
+  if (!buf[device]) {
+    unsigned* d = nullptr;
+    if (!ACF_CUDA_OK(cudaMalloc(&d, kTickets * sizeof(unsigned)))) return nullptr;
+    if (!ACF_CUDA_OK(cudaMemset(d, 0, kTickets * sizeof(unsigned)))) {
+      cudaFree(d);
+      return nullptr;
+    }
+    buf[device] = d;
+  }
+  return buf[device];
+}
+
+template <typename T, int DIM>
+bool stream_launch(Call& c, const AttnArgs& a) {
+  const int smem = (int)sizeof(StreamSmem<DIM>);
+  static int per_sm[64] = {};
+  const int dv = current_device() & 63;
+  if (!per_sm[dv]) {
+    int n = 0;
+    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_stream<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) ||
+        !ACF_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn_stream<T, DIM>, kWarps * 32, smem)))
+      return false;
+    per_sm[dv] = std::max(1, n);
+  }
+  StreamArgs p = {};
+  p.a = a;
+  const long long tiles = ((long long)std::min(a.b.max_new, a.b.tokens) * a.group + 15) / 16;
+  if (tiles * a.kv.heads > 0x7fffffffLL) {
+    set_error(kInvalid, "acfun_kv8_attention: too many rows");
+    return false;
+  }
+  p.row_tiles = (int)tiles;
+  // Split the keys so that one wave of resident blocks covers the batch; sequences of a batch may
+  // differ in length, and chunks of at most 1024 keys keep its longest from being the last.
+  const long long work = tiles * a.kv.heads * a.b.seqs;
+  const long long slots = (long long)per_sm[dv] * c.sm_count();
+  const long long want = std::max<long long>(1, slots / std::max<long long>(1, work));
+  long long chunk = (a.b.max_len + want - 1) / want;
+  if (a.b.seqs > 1) chunk = std::min<long long>(chunk, 1024);
+  chunk = std::max<long long>(chunk, kUnit * kWarps);
+  chunk = std::min<long long>((chunk + kUnit - 1) / kUnit * kUnit, (long long)(kMaxPages - 1) * a.kv.page);
+  p.chunk = (int)chunk;
+  p.splits = (int)((a.b.max_len + 2 * kUnit + chunk - 1) / chunk);
+  if (a.b.max_len <= chunk) p.splits = 1;
+  if (p.splits > 65535) {
+    set_error(kInvalid, "acfun_kv8_attention: max_len %d is too long for this page size", a.b.max_len);
+    return false;
+  }
+  if (p.splits > 1) {
+    const size_t n = (size_t)a.b.tokens * a.q_heads * p.splits;
+    p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
+    p.part_ml = (float2*)c.scratch(n * sizeof(float2));
+    if (work <= kTickets) {
+      p.tickets = tickets_of(current_device());
+    } else {
+      p.tickets = (unsigned*)c.scratch((size_t)work * sizeof(unsigned));
+      if (p.tickets && !ACF_CUDA_OK(cudaMemsetAsync(p.tickets, 0, (size_t)work * sizeof(unsigned), c.stream())))
+        return false;
+    }
+    if (!c.ok() || !p.tickets) return false;
+  }
+  k_attn_stream<T, DIM><<<dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), kWarps * 32, smem, c.stream()>>>(p, c.err());
+  return c.launched("k_attn_stream");
+}
+
+}  // namespace
+
+bool attn_stream_dev(Call& c, const AttnArgs& a) {
+  const int d = a.kv.dim;
+  if (a.dtype == ACFUN_F16)
+    return d == 64 ? stream_launch<__half, 64>(c, a) : d == 128 ? stream_launch<__half, 128>(c, a)
+                                                                 : stream_launch<__half, 256>(c, a);
+  return d == 64 ? stream_launch<__nv_bfloat16, 64>(c, a) : d == 128 ? stream_launch<__nv_bfloat16, 128>(c, a)
+                                                                      : stream_launch<__nv_bfloat16, 256>(c, a);
+}
+
+}  // namespace acf
+
+using namespace acf;
+
+extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatch* batch, const void* q, void* out,
+                                   int dtype, int q_heads, long long q_token, long long q_head, long long o_token,
+                                   long long o_head, float scale, int causal, int window, float* lse) {
+  const char* what = "acfun_kv8_attention";
+  if (int e = check_dtype(what, dtype, false)) return e;
+  if (int e = check_cache(what, cache)) return e;
+  if (int e = check_batch(what, batch, cache->page)) return e;
+  const int tokens = batch->tokens, dim = cache->dim;
+  if (q_heads <= 0 || q_heads % cache->heads) {
+    set_error(kInvalid, "%s: q_heads %d is not a positive multiple of the cache's %d heads", what, q_heads, cache->heads);
+    return kInvalid;
+  }
+  if (!isfinite(scale)) {
+    set_error(kInvalid, "%s: scale is not finite", what);
+    return kInvalid;
+  }
+  if (window < 0 || (window > 0 && !causal)) {
+    set_error(kInvalid, "%s: window %d must not be negative and needs causal", what, window);
+    return kInvalid;
+  }
+  if (int e = check_strides(what, q_token, q_head, tokens, q_heads, dim, false)) return e;
+  if (int e = check_strides(what, o_token, o_head, tokens, q_heads, dim, true)) return e;
+  if (batch->seqs == 0 || tokens == 0 || batch->max_new == 0) return 0;
+  if (!q || !out) {
+    set_error(kInvalid, "%s: q or out is NULL", what);
+    return kInvalid;
+  }
+  Call c(what);
+  if (!c.ok()) return last_error_code();
+  AttnArgs a = {};
+  a.kv = cache_view(cache);
+  a.b = batch_view(c, batch);
+  a.q = c.in(q, span_bytes(q_token, q_head, tokens, q_heads, dim, dtype));
+  a.out = c.inout(out, span_bytes(o_token, o_head, tokens, q_heads, dim, dtype));
+  a.lse = (float*)c.inout(lse, (size_t)tokens * q_heads * 4);
+  if (!c.ok()) return last_error_code();
+  a.q_token = q_token, a.q_head = q_head, a.o_token = o_token, a.o_head = o_head;
+  a.dtype = dtype, a.q_heads = q_heads, a.group = q_heads / cache->heads;
+  a.scale = scale, a.causal = causal != 0, a.window = window;
+  if (!attn_stream_dev(c, a)) c.fail();
+  return c.finish() ? 0 : last_error_code();
+}

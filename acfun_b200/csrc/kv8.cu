@@ -1,0 +1,465 @@
+// kv8.cu — the int8 key / value cache: tokens quantised into their pages (acfun_kv8_append), read
+// back as values (acfun_kv8_read), and the argument checks the cache's functions share.
+//
+// A scale covers the `page` tokens of one page and head, so one block sees all the new tokens of
+// a (page, head) and nothing is exchanged between blocks:
+//   s = max(max|x|, 127 * 2^-60) / 127, code = rint(x * (1 / s)) clamped to +-127;
+// in a page that holds older tokens s does not shrink, and when it grows, their codes are moved
+// to it in the same block.
+#include <algorithm>
+
+#include "attn.cuh"
+
+namespace acf {
+
+// ------------------------------------------------------------------ host checks
+int check_dtype(const char* what, int dtype, bool f32_ok) {
+  if (dtype == ACFUN_F16 || dtype == ACFUN_BF16 || (f32_ok && dtype == ACFUN_F32)) return 0;
+  set_error(kInvalid, "%s: dtype %d is not %sfp16 or bf16", what, dtype, f32_ok ? "fp32, " : "");
+  return kInvalid;
+}
+
+int check_cache(const char* what, const AcfunKvCache8* c) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) {
+    set_error(kInvalid, "%s: the cache or one of its arrays is NULL", what);
+    return kInvalid;
+  }
+  if (c->pages <= 0 || c->heads <= 0 || c->heads > 4096) {
+    set_error(kInvalid, "%s: pages %d must be positive and heads %d within [1, 4096]", what, c->pages, c->heads);
+    return kInvalid;
+  }
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) {
+    set_error(kInvalid, "%s: page %d is not 16, 32, 64 or 128", what, c->page);
+    return kInvalid;
+  }
+  if (c->dim != 64 && c->dim != 128 && c->dim != 256) {
+    set_error(kInvalid, "%s: dim %d is not 64, 128 or 256", what, c->dim);
+    return kInvalid;
+  }
+  if (!aligned16(c->k) || !aligned16(c->v) || ((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) {
+    set_error(kInvalid, "%s: codes must be 16-byte aligned, scales 4-byte aligned", what);
+    return kInvalid;
+  }
+  if (ptr_kind(c->k) != PtrKind::Device || ptr_kind(c->v) != PtrKind::Device ||
+      ptr_kind(c->k_scale) != PtrKind::Device || ptr_kind(c->v_scale) != PtrKind::Device) {
+    set_error(kInvalid, "%s: the cache must be device memory", what);
+    return kInvalid;
+  }
+  return 0;
+}
+
+int check_batch(const char* what, const AcfunKvBatch* b, int page) {
+  if (!b || b->seqs < 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->table_cols < 0) {
+    set_error(kInvalid, "%s: the batch is NULL or has a negative size", what);
+    return kInvalid;
+  }
+  if (b->seqs > 65535) {
+    set_error(kInvalid, "%s: %d sequences, at most 65535", what, b->seqs);
+    return kInvalid;
+  }
+  if (b->seqs > 0 && (!b->start || !b->length || (!b->table && b->table_cols > 0))) {
+    set_error(kInvalid, "%s: an index array of the batch is NULL", what);
+    return kInvalid;
+  }
+  if ((long long)b->table_cols * page < b->max_len) {
+    set_error(kInvalid, "%s: %d table columns of %d tokens do not reach max_len %d", what, b->table_cols, page,
+              b->max_len);
+    return kInvalid;
+  }
+  if (b->max_len > (1 << 30) || b->max_new > (1 << 30)) {
+    set_error(kInvalid, "%s: max_len and max_new are at most 2^30", what);
+    return kInvalid;
+  }
+  return 0;
+}
+
+int check_strides(const char* what, long long token, long long head, int tokens, int heads, int dim, bool output) {
+  const long long lim = 1LL << 46;
+  bool ok = token >= 0 && head >= 0 && token < lim && head < lim && (long long)heads * dim < (1LL << 27);
+  if (ok && output) {
+    const bool token_major = (tokens <= 1 || token >= (long long)(heads - 1) * head + dim) && (heads <= 1 || head >= dim);
+    const bool head_major = (heads <= 1 || head >= (long long)(tokens - 1) * token + dim) && (tokens <= 1 || token >= dim);
+    ok = token_major || head_major;
+  }
+  if (ok) return 0;
+  set_error(kInvalid, "%s: strides %lld (token) and %lld (head) of [%d, %d, %d] are negative, too large or overlap", what,
+            token, head, tokens, heads, dim);
+  return kInvalid;
+}
+
+KvView cache_view(const AcfunKvCache8* c) {
+  const int lg = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+  return {c->k, c->v, c->k_scale, c->v_scale, c->pages, c->heads, c->page, c->dim, lg};
+}
+
+BatchView batch_view(Call& c, const AcfunKvBatch* b) {
+  BatchView v = {};
+  v.table = (const int32_t*)c.in(b->table, (size_t)b->seqs * b->table_cols * 4);
+  v.start = (const int32_t*)c.in(b->start, ((size_t)b->seqs + 1) * 4);
+  v.length = (const int32_t*)c.in(b->length, (size_t)b->seqs * 4);
+  v.seqs = b->seqs, v.cols = b->table_cols, v.tokens = b->tokens, v.max_new = b->max_new, v.max_len = b->max_len;
+  return v;
+}
+
+namespace {
+
+// ------------------------------------------------------------------ append
+struct AppendArgs {
+  KvView kv;
+  BatchView b;
+  const void* k;
+  const void* v;
+  long long k_token, k_head, v_token, v_head;
+  int k_vec, v_vec;
+  const float* freq;
+  int rot, interleaved;
+  float amp;
+  int head_block;  // heads of one block
+};
+
+__device__ __forceinline__ float quant_fixup(float x) {
+  // NaN counts as 0, infinities as the largest finite value when coded
+  return x != x ? 0.0f : x;
+}
+__device__ __forceinline__ uint32_t code_of(float x, float unit) {
+  float r = rintf(__fmul_rn(x, unit));
+  r = fminf(fmaxf(r, -127.0f), 127.0f);
+  return (uint32_t)(int)r & 0xffu;
+}
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float unit) {
+  uint2 w = make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w.x |= code_of(x[i], unit) << (8 * i);
+    w.y |= code_of(x[4 + i], unit) << (8 * i);
+  }
+  return w;
+}
+
+// One block: page slot blockIdx.x of the new tokens of sequence blockIdx.z, heads
+// [blockIdx.y / 2 * head_block, ...), keys (blockIdx.y even) or values (odd).  A thread holds two
+// units of 16 elements of the tile in registers between the maximum and the coding: two runs of 8
+// elements, which in the half layout are the two sides of 8 pairs.  page * DIM / 32 threads.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigned* err) {
+  extern __shared__ float2 cs[];  // [tokens in this page][rot / 2], keys only
+  __shared__ float warp_max[2][32];
+  constexpr int UPR = DIM / 16;  // units per row
+  const int seq = blockIdx.z, page = a.kv.page;
+  const bool is_v = blockIdx.y & 1;
+  const SeqView sv = seq_view(a.b, seq, err);
+  const int first = sv.len - sv.n;  // position of the first new token
+  if (sv.n <= 0) return;
+  if (first < 0) {  // more new tokens than the sequence holds (or a length out of range)
+    if (threadIdx.x == 0) atomicOr(err, ACF_DEV_ERR_BADARG);
+    return;
+  }
+  const int g = first / page + blockIdx.x;           // this block's page of the sequence
+  if (g * (long long)page >= sv.len) return;
+  const int lo = max(first - g * page, 0), hi = min(sv.len - g * page, page);  // new slots [lo, hi)
+  const int row_of_slot0 = sv.row0 + g * page - first;  // packed row of slot 0 (may be before row0)
+  const int pid = seq_page(a.b, seq, g, a.kv.pages, err);
+  if (pid < 0) return;
+  const int h0 = (blockIdx.y >> 1) * a.head_block, h1 = min(h0 + a.head_block, a.kv.heads);
+  const int half = a.rot / 2;
+  const bool turn = !is_v && a.rot > 0;
+  if (turn) {
+    for (int i = threadIdx.x; i < (hi - lo) * half; i += blockDim.x) {
+      const int t = i / half;
+      cs[i] = rope_cs(g * page + lo + t, a.freq[i - t * half], a.amp);
+    }
+    __syncthreads();
+  }
+  // this thread's units: slot and the element offsets of their two runs
+  int slot[2], at0[2], at1[2], cs_at[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int idx = threadIdx.x + j * blockDim.x;
+    const int u = idx % UPR;
+    slot[j] = idx / UPR;
+    cs_at[j] = -1;
+    if (turn && !a.interleaved) {
+      const int pairs = a.rot / 16;
+      if (u < pairs) {
+        at0[j] = 8 * u, at1[j] = 8 * u + half;
+        cs_at[j] = (slot[j] - lo) * half + 8 * u;
+      } else {
+        at0[j] = a.rot + 16 * (u - pairs), at1[j] = at0[j] + 8;
+      }
+    } else {
+      at0[j] = 16 * u, at1[j] = 16 * u + 8;
+      if (turn && at0[j] < a.rot) cs_at[j] = (slot[j] - lo) * half + 8 * u;
+    }
+  }
+  const T* src = static_cast<const T*>(is_v ? a.v : a.k);
+  const long long tok_stride = is_v ? a.v_token : a.k_token, head_stride = is_v ? a.v_head : a.k_head;
+  const bool vec = is_v ? a.v_vec : a.k_vec;
+  int8_t* codes = is_v ? a.kv.v : a.kv.k;
+  float* scales = is_v ? a.kv.vs : a.kv.ks;
+
+  for (int h = h0; h < h1; ++h) {
+    float x[2][2][8];
+    float top = 127.0f * 0x1p-60f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (slot[j] >= lo && slot[j] < hi) {
+        const T* p = src + (long long)(row_of_slot0 + slot[j]) * tok_stride + h * head_stride;
+        load8(p + at0[j], vec, x[j][0]);
+        load8(p + at1[j], vec, x[j][1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[j][0][i] = x[j][1][i] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (slot[j] >= lo && slot[j] < hi && cs_at[j] >= 0) {
+        const float2* w = cs + cs_at[j];
+        if (a.interleaved) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 c = w[4 * r + i];
+              const float p = x[j][r][2 * i], q = x[j][r][2 * i + 1];
+              x[j][r][2 * i] = p * c.x - q * c.y;
+              x[j][r][2 * i + 1] = q * c.x + p * c.y;
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 c = w[i];
+            const float p = x[j][0][i], q = x[j][1][i];
+            x[j][0][i] = p * c.x - q * c.y;
+            x[j][1][i] = q * c.x + p * c.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[j][r][i] = quant_fixup(x[j][r][i]);
+          const float m = fabsf(x[j][r][i]);
+          if (m <= 3.4028234663852886e38f) top = fmaxf(top, m);
+        }
+    }
+    // block maximum; the buffers alternate so that one barrier per head is enough
+    float* wm = warp_max[h & 1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) wm[threadIdx.x >> 5] = top;
+    const size_t sc = (size_t)pid * a.kv.heads + h;
+    const float before = lo > 0 ? scales[sc] : 0.0f;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) top = fmaxf(top, wm[w]);
+    const float scale = fmaxf(before, __fdiv_rn(top, 127.0f));
+    const float unit = __frcp_rn(scale);
+    int8_t* tile = codes + sc * page * DIM;
+    if (scale > before && lo > 0) {  // older tokens of the page move to the larger scale
+      const float f = __fdiv_rn(before, scale);
+      for (int i = threadIdx.x; i < lo * (DIM / 4); i += blockDim.x) {
+        uint32_t w = reinterpret_cast<uint32_t*>(tile)[i], r = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) r |= code_of((float)(int8_t)(w >> (8 * b)), f) << (8 * b);
+        reinterpret_cast<uint32_t*>(tile)[i] = r;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (slot[j] < lo || slot[j] >= hi) continue;
+      int8_t* o = tile + slot[j] * DIM;
+      const uint2 w0 = codes8(x[j][0], unit), w1 = codes8(x[j][1], unit);
+      if (at1[j] == at0[j] + 8) {
+        *reinterpret_cast<uint4*>(o + at0[j]) = make_uint4(w0.x, w0.y, w1.x, w1.y);
+      } else {
+        *reinterpret_cast<uint2*>(o + at0[j]) = w0;
+        *reinterpret_cast<uint2*>(o + at1[j]) = w1;
+      }
+    }
+    // every thread has read the old scale before the barrier above
+    if (threadIdx.x == 0) scales[sc] = scale;
+  }
+  // new tokens past the last page slot of the grid
+  if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1 && (g + 1) * (long long)page < sv.len)
+    atomicOr(err, ACF_DEV_ERR_BADARG);
+}
+
+template <typename T, int DIM>
+bool append_launch(Call& c, AppendArgs a) {
+  const int page = a.kv.page;
+  const int threads = page * DIM / 32;
+  // pages that a run of max_new tokens can touch
+  const int slots = std::max(1, (std::min(a.b.max_new, a.b.max_len) + page - 2) / page + 1);
+  // All heads of a page in one block share its cosines and sines; with few pages the heads go to
+  // blocks of their own, which recompute them but fill the machine.
+  const long long pages = (long long)slots * a.b.seqs;
+  int parts = (int)std::min<long long>(a.kv.heads, std::max<long long>(1, 4LL * c.sm_count() / std::max<long long>(1, pages)));
+  a.head_block = (a.kv.heads + parts - 1) / parts;
+  parts = (a.kv.heads + a.head_block - 1) / a.head_block;
+  const size_t smem = (size_t)std::min(page, a.b.max_new) * (a.rot / 2) * sizeof(float2);
+  static bool attr_done[64] = {false};
+  const int dv = current_device();
+  if (smem > 48 * 1024 && !attr_done[dv & 63]) {
+    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_kv8_append<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          128 * (DIM / 2) * (int)sizeof(float2))))
+      return false;
+    attr_done[dv & 63] = true;
+  }
+  k_kv8_append<T, DIM><<<dim3(slots, 2 * parts, a.b.seqs), threads, smem, c.stream()>>>(a, c.err());
+  return c.launched("k_kv8_append");
+}
+
+// ------------------------------------------------------------------ read
+struct ReadArgs {
+  KvView kv;
+  BatchView b;
+  void* k;
+  void* v;
+  int head_block;
+};
+
+// One block: page slot blockIdx.x of the tokens wanted of sequence blockIdx.z, `head_block` heads
+// of it.  Codes of neighbouring heads are contiguous; a thread turns 16 codes into values.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(256) k_kv8_read(const ReadArgs a, unsigned* err) {
+  const int seq = blockIdx.z, page = a.kv.page;
+  const SeqView sv = seq_view(a.b, seq, err);
+  const int first = sv.len - sv.n;
+  if (sv.n <= 0) return;
+  if (first < 0) {
+    if (threadIdx.x == 0) atomicOr(err, ACF_DEV_ERR_BADARG);
+    return;
+  }
+  const int g = first / page + blockIdx.x;
+  if (g * (long long)page >= sv.len) return;
+  const int lo = max(first - g * page, 0), hi = min(sv.len - g * page, page);
+  const int pid = seq_page(a.b, seq, g, a.kv.pages, err);
+  if (pid < 0) return;
+  if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1 && (g + 1) * (long long)page < sv.len)
+    atomicOr(err, ACF_DEV_ERR_BADARG);
+  const int h0 = blockIdx.y * a.head_block, nh = min(a.head_block, a.kv.heads - h0);
+  constexpr int CPR = DIM / 16;  // 16-code runs per row
+  const int rows = hi - lo, total = nh * rows * CPR;
+  const size_t head0 = (size_t)pid * a.kv.heads + h0;
+  const long long out0 = (long long)(sv.row0 + g * page + lo - first) * a.kv.heads + h0;
+  for (int i = threadIdx.x; i < total; i += blockDim.x) {
+    const int c = i % CPR, rest = i / CPR, r = rest % rows, h = rest / rows;
+    const size_t from = (((head0 + h) * page) + lo + r) * DIM + 16 * c;
+    const size_t to = (size_t)(out0 + (long long)r * a.kv.heads + h) * DIM + 16 * c;
+    uint4 wk = {}, wv = {};
+    float sk = 0.f, sv_ = 0.f;
+    if (a.k) wk = *reinterpret_cast<const uint4*>(a.kv.k + from), sk = a.kv.ks[head0 + h];
+    if (a.v) wv = *reinterpret_cast<const uint4*>(a.kv.v + from), sv_ = a.kv.vs[head0 + h];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      T* o = static_cast<T*>(which ? a.v : a.k);
+      if (!o) continue;
+      const uint4 w = which ? wv : wk;
+      const float s = which ? sv_ : sk;
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)(words[2 * e + j / 4] >> (8 * (j % 4))) * s;
+        store8(o + to + 8 * e, true, x);
+      }
+    }
+  }
+}
+
+template <typename T, int DIM>
+bool read_launch(Call& c, ReadArgs a) {
+  const int page = a.kv.page;
+  const int slots = std::max(1, (std::min(a.b.max_new, a.b.max_len) + page - 2) / page + 1);
+  // a block takes the heads that make about two passes of its 256 threads
+  a.head_block = std::max(1, std::min(a.kv.heads, 512 * 16 / (page * DIM)));
+  const int parts = (a.kv.heads + a.head_block - 1) / a.head_block;
+  k_kv8_read<T, DIM><<<dim3(slots, parts, a.b.seqs), 256, 0, c.stream()>>>(a, c.err());
+  return c.launched("k_kv8_read");
+}
+
+template <typename F16, typename BF16, typename F32>
+bool by_dtype(int dtype, F16 f16, BF16 bf16, F32 f32) {
+  return dtype == ACFUN_F16 ? f16() : dtype == ACFUN_BF16 ? bf16() : f32();
+}
+
+}  // namespace
+}  // namespace acf
+
+using namespace acf;
+
+#define ACF_BY_DIM(fn, T, args) \
+  (args.kv.dim == 64 ? fn<T, 64>(c, args) : args.kv.dim == 128 ? fn<T, 128>(c, args) : fn<T, 256>(c, args))
+#define ACF_BY_DTYPE(fn, dtype, args)                        \
+  by_dtype(dtype, [&] { return ACF_BY_DIM(fn, __half, args); }, \
+           [&] { return ACF_BY_DIM(fn, __nv_bfloat16, args); }, [&] { return ACF_BY_DIM(fn, float, args); })
+
+extern "C" int acfun_kv8_append(const AcfunKvCache8* cache, const AcfunKvBatch* batch, const void* k, const void* v,
+                                int dtype, long long k_token, long long k_head, long long v_token, long long v_head,
+                                const AcfunRope* rope) {
+  const char* what = "acfun_kv8_append";
+  if (int e = check_dtype(what, dtype, true)) return e;
+  if (int e = check_cache(what, cache)) return e;
+  if (int e = check_batch(what, batch, cache->page)) return e;
+  if (rope) {
+    if (int e = check_rope(what, rope, cache->dim)) return e;
+    if (rope->rot % 16) {
+      set_error(kInvalid, "%s: rope.rot %d is not a multiple of 16 (rotate such keys with acfun_rope first)", what,
+                rope->rot);
+      return kInvalid;
+    }
+  }
+  const int heads = cache->heads, dim = cache->dim, tokens = batch->tokens;
+  if (int e = check_strides(what, k_token, k_head, tokens, heads, dim, false)) return e;
+  if (int e = check_strides(what, v_token, v_head, tokens, heads, dim, false)) return e;
+  if (batch->seqs == 0 || tokens == 0 || batch->max_new == 0) return 0;
+  if (!k || !v) {
+    set_error(kInvalid, "%s: k or v is NULL", what);
+    return kInvalid;
+  }
+  Call c(what);
+  if (!c.ok()) return last_error_code();
+  AppendArgs a = {};
+  a.kv = cache_view(cache);
+  a.b = batch_view(c, batch);
+  a.k = c.in(k, span_bytes(k_token, k_head, tokens, heads, dim, dtype));
+  a.v = c.in(v, span_bytes(v_token, v_head, tokens, heads, dim, dtype));
+  if (rope && rope->rot) {
+    a.freq = (const float*)c.in(rope->freq, (size_t)rope->rot / 2 * 4);
+    a.rot = rope->rot, a.interleaved = rope->interleaved != 0, a.amp = rope->amplitude;
+  }
+  if (!c.ok()) return last_error_code();
+  const long long per16 = 16 / (long long)dtype_size(dtype);
+  a.k_vec = aligned16(a.k) && k_token % per16 == 0 && k_head % per16 == 0;
+  a.v_vec = aligned16(a.v) && v_token % per16 == 0 && v_head % per16 == 0;
+  a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+  if (!ACF_BY_DTYPE(append_launch, dtype, a)) c.fail();
+  return c.finish() ? 0 : last_error_code();
+}
+
+extern "C" int acfun_kv8_read(const AcfunKvCache8* cache, const AcfunKvBatch* batch, void* k, void* v, int dtype) {
+  const char* what = "acfun_kv8_read";
+  if (int e = check_dtype(what, dtype, true)) return e;
+  if (int e = check_cache(what, cache)) return e;
+  if (int e = check_batch(what, batch, cache->page)) return e;
+  if (batch->seqs == 0 || batch->tokens == 0 || batch->max_new == 0 || (!k && !v)) return 0;
+  Call c(what);
+  if (!c.ok()) return last_error_code();
+  ReadArgs a = {};
+  a.kv = cache_view(cache);
+  a.b = batch_view(c, batch);
+  const size_t bytes = (size_t)batch->tokens * cache->heads * cache->dim * dtype_size(dtype);
+  // rows of a sequence that is skipped keep what they held
+  a.k = c.inout(k, bytes);
+  a.v = c.inout(v, bytes);
+  if (!c.ok()) return last_error_code();
+  if ((a.k && !aligned16(a.k)) || (a.v && !aligned16(a.v))) {
+    set_error(kInvalid, "%s: k and v must be 16-byte aligned", what);
+    c.fail();
+  } else if (!ACF_BY_DTYPE(read_launch, dtype, a)) {
+    c.fail();
+  }
+  return c.finish() ? 0 : last_error_code();
+}

@@ -1,0 +1,207 @@
+"""Rotary positions and attention over an int8 paged key / value cache (acfun_rope, acfun_kv8_*).
+
+Activations are torch tensors or numpy arrays [tokens, heads, dim] whose last dimension is
+contiguous (fp32, fp16 or bf16; numpy has no bf16); the cache is a set of CUDA tensors.  Calls
+on device tensors are stream-ordered on the library's stream, as everywhere in this package.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import AcfunError, check, lib
+
+_DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_codes = {}
+
+
+def _dtype_code(dt):
+    code = _codes.get(dt)
+    if code is None:
+        code = _DTYPES.get(str(dt).replace("torch.", ""))
+        if code is None:
+            raise TypeError(f"dtype {dt} is not float32, float16 or bfloat16")
+        _codes[dt] = code
+    return code
+
+
+class _Cache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int), ("heads", C.c_int), ("page", C.c_int), ("dim", C.c_int)]
+
+
+class _Batch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("start", C.c_void_p), ("length", C.c_void_p), ("seqs", C.c_int),
+                ("table_cols", C.c_int), ("tokens", C.c_int), ("max_new", C.c_int), ("max_len", C.c_int)]
+
+
+class _Rope(C.Structure):
+    _fields_ = [("freq", C.c_void_p), ("rot", C.c_int), ("interleaved", C.c_int), ("amplitude", C.c_float)]
+
+
+def _address(x):
+    return x.ctypes.data if isinstance(x, np.ndarray) else x.data_ptr()
+
+
+def _flat(x, dtype, what):
+    """The address of a contiguous array of the given element type."""
+    if isinstance(x, np.ndarray):
+        ok = x.flags["C_CONTIGUOUS"] and x.dtype.name == dtype
+    else:
+        ok = x.is_contiguous() and str(x.dtype) == "torch." + dtype
+    if not ok:
+        raise ValueError(f"{what} must be contiguous {dtype}")
+    return _address(x)
+
+
+def _strides(x, what):
+    """(token, head) strides in elements of [tokens, heads, dim]."""
+    if x.ndim != 3:
+        raise ValueError(f"{what} must be [tokens, heads, dim], got {tuple(x.shape)}")
+    if isinstance(x, np.ndarray):
+        t, h, d = (s // x.itemsize for s in x.strides)
+    else:
+        t, h, d = x.stride()
+    if d != 1 and x.shape[2] != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    return t, h
+
+
+def _empty(like, shape, dtype=None):
+    if isinstance(like, np.ndarray):
+        return np.empty(shape, dtype=dtype or like.dtype)
+    import torch
+    return torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
+
+
+def _done(code):
+    if code:
+        check()
+        raise AcfunError(f"acfun error {code}")
+
+
+class Rope:
+    """Rotary positions: pair i of a head's first 2 * len(freq) elements turns by position *
+    freq[i]; freq is fp32 and is kept by reference.  See rope_frequencies()."""
+
+    def __init__(self, freq, interleaved=False, amplitude=1.0):
+        if freq.ndim != 1:
+            raise ValueError("freq must have one dimension")
+        self.freq = freq
+        self.c = _Rope(_flat(freq, "float32", "freq"), 2 * freq.shape[0], int(bool(interleaved)), float(amplitude))
+        self.ref = C.byref(self.c)
+
+
+def rope_frequencies(rot, base=10000.0, scaling=None, factor=1.0, trained=0, fast=32.0, slow=1.0):
+    """(freq, amplitude): numpy fp32 [rot / 2] and a float.  scaling: None; "linear" (positions
+    divided by factor); "base" (base enlarged so that the lowest frequency is divided by factor);
+    "by_parts" or "by_turns" (frequencies kept, divided or mixed by how often a pair turns within the
+    `trained` length: above `fast` turns, below `slow`, between; mixed linearly in the pair's index
+    or in the turns)."""
+    kinds = {None: 0, "linear": 1, "base": 2, "by_parts": 3, "by_turns": 4}
+    if scaling not in kinds:
+        raise ValueError(f"scaling {scaling!r} is not one of {sorted(k for k in kinds if k)}")
+    if rot <= 0:
+        raise ValueError("rot must be positive")
+    freq = np.empty(rot // 2, np.float32)
+    amp = C.c_float()
+    _done(lib().acfun_rope_frequencies(rot, base, kinds[scaling], factor, trained, fast, slow, freq.ctypes.data,
+                                       C.byref(amp)))
+    return freq, amp.value
+
+
+def rope(x, positions, spec: Rope, out=None):
+    """x [tokens, heads, dim] at int32 positions [tokens]; out may be x."""
+    t, h = _strides(x, "x")
+    if positions.shape != (x.shape[0],):
+        raise ValueError("positions must be [tokens]")
+    if out is None:
+        out = _empty(x, x.shape)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("out must have x's shape and dtype")
+    ot, oh = _strides(out, "out")
+    _done(lib().acfun_rope(_address(x), _address(out), _dtype_code(x.dtype), x.shape[0], x.shape[1], x.shape[2], t, h,
+                           ot, oh, _flat(positions, "int32", "positions"), spec.ref))
+    return out
+
+
+class KvBatch:
+    """Sequences of one step: table int32 [seqs, columns] of page numbers, start int32 [seqs + 1]
+    (offsets of the sequences' new tokens in the packed activations), length int32 [seqs] (tokens
+    in the cache, the new ones last), and on the host the number of packed tokens and bounds on
+    any sequence's new tokens and length.  The arrays are kept by reference and read when a call's
+    kernels run."""
+
+    def __init__(self, table, start, length, tokens, max_new, max_len):
+        if table.ndim != 2 or length.shape != (table.shape[0],) or start.shape != (table.shape[0] + 1,):
+            raise ValueError("table must be [seqs, columns], start [seqs + 1] and length [seqs]")
+        self.arrays = (table, start, length)
+        self.tokens = int(tokens)
+        self.c = _Batch(_flat(table, "int32", "table"), _flat(start, "int32", "start"),
+                        _flat(length, "int32", "length"), table.shape[0], table.shape[1], self.tokens, int(max_new),
+                        int(max_len))
+        self.ref = C.byref(self.c)
+
+
+class KvCache8:
+    """Keys and values as int8 codes [pages, heads, page, dim] with fp32 scales [pages, heads] (CUDA
+    tensors, kept by reference)."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.ndim != 4 or v.shape != k.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+            raise ValueError("codes must be [pages, heads, page, dim], scales [pages, heads]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.heads, self.page, self.dim = k.shape
+        self.c = _Cache(_flat(k, "int8", "k"), _flat(v, "int8", "v"), _flat(k_scale, "float32", "k_scale"),
+                        _flat(v_scale, "float32", "v_scale"), *k.shape)
+        self.ref = C.byref(self.c)
+
+    @classmethod
+    def empty(cls, pages, heads, dim, page=64, device="cuda"):
+        """A cache of `pages` unwritten pages."""
+        import torch
+        codes = [torch.zeros((pages, heads, page, dim), dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros((pages, heads), dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+    def _new(self, x, batch, what):
+        if tuple(x.shape) != (batch.tokens, self.heads, self.dim):
+            raise ValueError(f"{what} must be [{batch.tokens}, {self.heads}, {self.dim}], got {tuple(x.shape)}")
+        return _strides(x, what)
+
+    def append(self, k, v, batch: KvBatch, rope: Rope | None = None):
+        """Quantise the batch's new keys (rotated by their position in the sequence when rope is
+        given) and values into their pages."""
+        kt, kh = self._new(k, batch, "k")
+        vt, vh = self._new(v, batch, "v")
+        if k.dtype != v.dtype:
+            raise ValueError("k and v must have one dtype")
+        _done(lib().acfun_kv8_append(self.ref, batch.ref, _address(k), _address(v), _dtype_code(k.dtype), kt, kh, vt,
+                                     vh, rope.ref if rope is not None else None))
+
+    def read(self, batch: KvBatch, dtype):
+        """(k, v) [tokens, heads, dim]: the last start[i + 1] - start[i] tokens of each sequence."""
+        shape = (batch.tokens, self.heads, self.dim)
+        k, v = _empty(self.k, shape, dtype), _empty(self.k, shape, dtype)
+        _done(lib().acfun_kv8_read(self.ref, batch.ref, k.data_ptr(), v.data_ptr(), _dtype_code(dtype)))
+        return k, v
+
+    def attention(self, q, batch: KvBatch, scale=None, causal=True, window=0, out=None, lse=None):
+        """softmax(scale * q k^T) v for q [tokens, q_heads, dim]; scale defaults to dim ** -0.5.  lse
+        (fp32 [tokens, q_heads]) receives the logarithm of the softmax denominators."""
+        qt, qh = _strides(q, "q")
+        if q.shape[0] != batch.tokens or q.shape[2] != self.dim:
+            raise ValueError(f"q must be [{batch.tokens}, q_heads, {self.dim}], got {tuple(q.shape)}")
+        if out is None:
+            out = _empty(q, q.shape)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must have q's shape and dtype")
+        if lse is not None and tuple(lse.shape) != tuple(q.shape[:2]):
+            raise ValueError("lse must be [tokens, q_heads]")
+        ot, oh = _strides(out, "out")
+        _done(lib().acfun_kv8_attention(self.ref, batch.ref, _address(q), _address(out), _dtype_code(q.dtype),
+                                        q.shape[1], qt, qh, ot, oh, self.dim ** -0.5 if scale is None else scale,
+                                        int(bool(causal)), window,
+                                        _flat(lse, "float32", "lse") if lse is not None else None))
+        return out

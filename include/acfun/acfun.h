@@ -162,6 +162,88 @@ int acfun_gemm_epi_noalloc(int M, int N, int K, const float* A, const float* B, 
  * mode).  Process-wide. */
 int acfun_set_fp32_math(int mode);
 
+/* ---- attention over an int8 key / value cache (no reference counterpart) ----
+ *
+ * The pieces of a decoder block between its projections: rotary positions, a paged cache that
+ * holds keys and values as int8 codes, and attention that reads the codes.  Activations are
+ * fp32, fp16 or bf16 (`dtype`); a tensor [tokens, heads, dim] is given by its address and its
+ * token and head strides in elements (dim is contiguous), so a slice of a packed q/k/v row can
+ * be passed in place.  All functions return 0 or an error code (also in acfun_last_error()) and
+ * check their arguments on the host; entries of device arrays (table, start, length) are checked
+ * in the kernels: a bad one skips its sequence and is reported, as code 1, by the next
+ * acfun_synchronize().  Activations and index arrays may be host memory; the cache itself must be
+ * device memory. */
+#define ACFUN_F32 0
+#define ACFUN_F16 1
+#define ACFUN_BF16 2
+
+/* Codes [pages][heads][page][dim] and one scale per (page, head): value = code * scale.
+ * page is 16, 32, 64 or 128 tokens; dim is 64, 128 or 256. */
+typedef struct AcfunKvCache8 {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale; /* [pages][heads] */
+  float* v_scale;
+  int pages, heads, page, dim;
+} AcfunKvCache8;
+
+/* A batch of sequences.  Sequence i has length[i] tokens in the cache, token j of it in page
+ * table[i * table_cols + j / page] at slot j % page.  Its new tokens are its last ones,
+ * start[i+1] - start[i] of them, rows start[i].. of the packed activations.  max_new and max_len
+ * bound the new tokens and the length of any sequence; tokens is start[seqs]. */
+typedef struct AcfunKvBatch {
+  const int32_t* table;
+  const int32_t* start;  /* [seqs + 1] */
+  const int32_t* length; /* [seqs] */
+  int seqs, table_cols, tokens, max_new, max_len;
+} AcfunKvBatch;
+
+/* Rotary positions: pair i of the first `rot` elements of a head turns by pos * freq[i] and is
+ * scaled by amplitude; the elements after them are copied.  Pairs are (i, i + rot/2), or
+ * (2i, 2i + 1) when interleaved. */
+typedef struct AcfunRope {
+  const float* freq; /* [rot / 2] */
+  int rot, interleaved;
+  float amplitude;
+} AcfunRope;
+
+/* Frequencies base^(-2i/rot) for i < rot/2, adapted to contexts `factor` times as long as the
+ * `trained` one, written to host memory, and the amplitude that goes with them (may be NULL):
+ *   0  none
+ *   1  positions divided by factor
+ *   2  base enlarged by factor^(rot/(rot-2)), so the lowest frequency is divided by factor
+ *   3  by wavelength: pairs that turn more than `fast` times in the trained length keep their
+ *      frequency, those below `slow` turns are divided by factor, linear in the pair's index
+ *      between; amplitude 0.1 ln(factor) + 1
+ *   4  as 3, linear in the number of turns between, amplitude 1 */
+int acfun_rope_frequencies(int rot, double base, int scaling, double factor, double trained,
+                           double fast, double slow, float* freq, float* amplitude);
+/* y = x with positions pos[token] in [0, 2^31) applied; rot even and at most dim; y may be x. */
+int acfun_rope(const void* x, void* y, int dtype, int tokens, int heads, int dim,
+               long long x_token, long long x_head, long long y_token, long long y_head,
+               const int32_t* pos, const AcfunRope* rope);
+/* Quantise the batch's new keys and values into the cache; keys are rotated by their position in
+ * the sequence first when rope is given (rot a multiple of 16).  The scale of a (page, head) is
+ * max(max|x|, 127 * 2^-60) / 127 over the new tokens in the page, code = rint(x * (1 / scale))
+ * clamped to +-127.  A page that holds older tokens keeps the larger of its scale and the new
+ * one, and when that grows, older codes become rint(code * (old / new)).  Infinities saturate
+ * to +-127 and NaN becomes 0; neither enters a scale.  Pages written must not be shared between
+ * sequences. */
+int acfun_kv8_append(const AcfunKvCache8* cache, const AcfunKvBatch* batch, const void* k, const void* v,
+                     int dtype, long long k_token, long long k_head, long long v_token, long long v_head,
+                     const AcfunRope* rope);
+/* The batch's last start[i+1] - start[i] tokens as values, k and v [tokens, heads, dim] contiguous
+ * (either may be NULL). */
+int acfun_kv8_read(const AcfunKvCache8* cache, const AcfunKvBatch* batch, void* k, void* v, int dtype);
+/* out = softmax(scale * q k^T) v over each sequence's cached tokens.  q and out are [tokens,
+ * q_heads, dim] in fp16 or bf16, q head h reads cache head h / (q_heads / heads).  causal: a new
+ * token sees the tokens up to itself, and with window > 0 only the last `window` of them.  A row
+ * that sees nothing is 0.  lse (fp32 [tokens, q_heads], may be NULL) is the natural logarithm of
+ * the softmax denominator, -inf for a row that sees nothing. */
+int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatch* batch, const void* q, void* out,
+                        int dtype, int q_heads, long long q_token, long long q_head, long long o_token,
+                        long long o_head, float scale, int causal, int window, float* lse);
+
 /* Stream for device-pointer calls (a cudaStream_t passed as void*; NULL = legacy default). */
 void acfun_set_stream(void* stream);
 void* acfun_get_stream(void);
