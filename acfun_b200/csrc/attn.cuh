@@ -164,6 +164,8 @@ struct AttnArgs {
   float scale;
   int causal, window;
 };
-bool attn_stream_dev(Call& c, const AttnArgs& a);
+bool attn_stream_dev(Call& c, const AttnArgs& a);  // any shape
+bool attn_tc_dev(Call& c, const AttnArgs& a);      // where attn_tc_takes
+bool attn_tc_takes(const AttnArgs& a);
 
 }  // namespace acf

@@ -25,7 +25,7 @@
 
 #include <algorithm>
 
-#include "attn.cuh"
+#include "attn_tile.cuh"
 
 namespace acf {
 namespace {
@@ -33,10 +33,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;          // keys per step of a warp
 constexpr int kMaxPages = 1024;    // pages of one chunk (their scales are staged in shared memory)
-// Weights are kept within fp16's upper range, so that keys far below the largest keep their bits:
-// a row's offset m is set so that its largest weight is 2^kTop, and moves when one would pass
-// 2^kMost.
-constexpr float kTop = 7.0f, kMost = 15.0f;
 constexpr int kTickets = 1 << 16;
 
 struct StreamArgs {
@@ -55,10 +51,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
@@ -121,9 +113,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
   const int nr = min(16, rows - r0);
   const int t_first = r0 / a.group, t_last = (r0 + nr - 1) / a.group;
   const int pos0 = sv.len - sv.n;  // position of new token 0 (negative: it sees nothing)
-  const int key_hi = a.causal ? max(0, min(sv.len, pos0 + t_last + 1)) : sv.len;
-  const int key_lo = a.window > 0 ? max(0, pos0 + t_first - a.window + 1) : 0;
-  const int unit0 = key_lo / kUnit, units = key_hi > key_lo ? (key_hi + kUnit - 1) / kUnit - unit0 : 0;
+  const KeyRange kr = key_range(a, sv, r0, nr, kUnit);
+  const int unit0 = kr.first, units = kr.n;
   const int per = p.chunk / kUnit;
   const int nsplit = max(1, (units + per - 1) / per);
   if (chunk_i >= nsplit) return;
@@ -200,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   __syncthreads();
 
-  uint4 kr[2][KR];
+  uint4 kc[2][KR];
   uint32_t vr[4][VW];
   auto place = [&](int u) -> size_t {  // byte offset of the unit's first key, this head
     const PageEntry& e = sm.pages[((u * kUnit) >> lg) - pg0];
@@ -212,7 +203,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < KR; ++r) kr[t][r] = ldg16(b + t * 8 * DIM + r * 64);
+      for (int r = 0; r < KR; ++r) kc[t][r] = ldg16(b + t * 8 * DIM + r * 64);
   };
   auto load_v = [&](int u) {
     const int8_t* b = a.kv.v + place(u) + g * (DIM / 8);
@@ -245,7 +236,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < KR; ++r) {
-        const uint32_t w[4] = {kr[t][r].x, kr[t][r].y, kr[t][r].z, kr[t][r].w};
+        const uint32_t w[4] = {kc[t][r].x, kc[t][r].y, kc[t][r].z, kc[t][r].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t x = w[i] ^ 0x80808080u;
@@ -516,6 +507,6 @@ extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatc
   a.q_token = q_token, a.q_head = q_head, a.o_token = o_token, a.o_head = o_head;
   a.dtype = dtype, a.q_heads = q_heads, a.group = q_heads / cache->heads;
   a.scale = scale, a.causal = causal != 0, a.window = window;
-  if (!attn_stream_dev(c, a)) c.fail();
+  if (!(attn_tc_takes(a) ? attn_tc_dev(c, a) : attn_stream_dev(c, a))) c.fail();
   return c.finish() ? 0 : last_error_code();
 }

@@ -1,0 +1,563 @@
+// attn_kv8_tc.cu — attention over the int8 cache on the tcgen05 tensor cores, for calls with many
+// rows per cache head (prompts, chunks of prompts, batches of drafts).
+//
+// Rows are packed as in attn_kv8.cu (row = token * group + head of the group), 256 to a block: two
+// tiles of 128, A and B, against the same keys.  Per 128 keys and tile
+//   S = Q K^T  (M = 128, N = 128, both operands fp16 in shared memory)  -> TMEM
+//   w = 2^(S f + log2 s_v - m) in registers, one row per thread, rounded to fp16 -> TMEM, over S
+//   O += w V   (A operand from TMEM, V's codes as fp16 in shared memory, N = dim)  -> TMEM
+// so the tensor cores work on one tile while the other is in its softmax.  Codes are exact in fp16;
+// K scales, V scales and q's power of two enter the exponent as in attn_kv8.cu, and the running
+// offset m moves only when a weight would pass 2^15, so O is rescaled a few times per row at most.
+//
+//   warps 0-3, 4-7  Q of tile A / B to shared memory, then its softmax and output (a TMEM lane and
+//                   a row per thread)
+//   warps 8-11      codes from global memory, one tile ahead in registers, to fp16 in the 128-byte
+//                   swizzled layout of the MMA operands; two stages each for K and V
+//   warp 12         the MMA issuer; warps 13-15 only lend their registers
+// TMEM: S of A and B (128 columns each; the fp16 weights overlay their first half), O of A and B.
+// Every wait is bounded (ptx.cuh); on expiry the error word is set and all roles leave.
+#include <math.h>
+
+#include <algorithm>
+
+#include "attn_tile.cuh"
+
+namespace acf {
+namespace {
+
+constexpr int kTcThreads = 512;
+constexpr int kRows = 256;     // packed rows of a block
+constexpr int kKeys = 128;     // keys per step
+constexpr int kUnits = kKeys / 16;
+constexpr float kLeast = 1e-37f;  // a factor never underflows to 0: a masked score stays -inf under it
+constexpr int kScaleRing = 4;  // the converters are at most two tiles ahead of a softmax
+
+struct TcArgs {
+  AttnArgs a;
+  int chunk;       // key tiles per block
+  int splits;
+  float* part_o;   // [tokens][q_heads][splits][DIM], null when splits == 1
+  float2* part_ml;
+  int row_tiles;
+};
+
+template <int DIM>
+struct TcSmem {
+  static constexpr int kChunks = DIM / 64;               // 128-byte column chunks
+  static constexpr int kQTile = 128 * DIM * 2;
+  static constexpr int kTile = kKeys * DIM * 2;          // one stage of K or V
+  static constexpr int kQ = 0, kK = 2 * kQTile, kV = kK + 2 * kTile, kBars = kV + 2 * kTile;
+  static constexpr int kScales = kBars + 256;
+  static constexpr int kBytes = kScales + kScaleRing * kUnits * 16 + 1024;  // + alignment
+  static_assert(kBytes <= 232448, "shared memory");
+};
+
+struct TcBars {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_full, drain;
+  uint32_t tmem;
+  volatile int abort;
+};
+static_assert(sizeof(TcBars) <= 256, "barrier block");
+
+__device__ __forceinline__ void umma_ts_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// 32 consecutive columns of this warp's lanes; r points into a register array.
+__device__ __forceinline__ void tmem_ld32p(uint32_t t, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(t));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 codes to fp16, written as two 16-byte units of row `row` of a swizzled operand tile: code
+// chunk c (16 codes) of the row lies in column chunk c / 4.
+__device__ __forceinline__ void put_codes(uint8_t* tile, int row, int c, uint4 w) {
+  const uint32_t in[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+  uint8_t* base = tile + (c >> 2) * (kKeys * 128) + row * 128;
+  const int u = 2 * (c & 3), x = row & 7;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint4 o;
+    o.x = f16_from_u8(in[2 * h], 0x4140), o.y = f16_from_u8(in[2 * h], 0x4342);
+    o.z = f16_from_u8(in[2 * h + 1], 0x4140), o.w = f16_from_u8(in[2 * h + 1], 0x4342);
+    *reinterpret_cast<uint4*>(base + (((u + h) ^ x) << 4)) = o;
+  }
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsigned* err) {
+  using L = TcSmem<DIM>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TcBars& bar = *reinterpret_cast<TcBars*>(smem + L::kBars);
+  float4* scales = reinterpret_cast<float4*>(smem + L::kScales);  // [ring][unit]: k factor, log2 v, 1 / v
+  const AttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // late row tiles see the most keys when causal: they go first
+  const int head = blockIdx.x % a.kv.heads, rt = p.row_tiles - 1 - blockIdx.x / a.kv.heads;
+  const int seq = blockIdx.y, part = blockIdx.z;
+  const SeqView sv = seq_view(a.b, seq, err);
+  const int rows = sv.n * a.group, r0 = rt * kRows;
+  if (r0 >= rows) return;
+  const int nr = min(kRows, rows - r0);
+  const KeyRange kr = key_range(a, sv, r0, nr, kKeys);
+  const int nsplit = max(1, (kr.n + p.chunk - 1) / p.chunk);
+  if (part >= nsplit) return;
+  const int tile0 = kr.first + part * p.chunk, ntiles = min(kr.n - part * p.chunk, p.chunk);
+  const bool two = nr > 128;
+
+  if (threadIdx.x == 0) {
+    dev::mbar_init(&bar.q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      dev::mbar_init(&bar.k_full[i], 128);
+      dev::mbar_init(&bar.k_empty[i], 1);
+      dev::mbar_init(&bar.v_full[i], 128);
+      dev::mbar_init(&bar.v_empty[i], 1);
+      dev::mbar_init(&bar.s_full[i], 1);
+      dev::mbar_init(&bar.p_full[i], 128);
+    }
+    dev::mbar_init(&bar.o_full, 1);
+    dev::mbar_init(&bar.drain, 1);
+    bar.abort = 0;
+    dev::fence_mbar_init();
+  }
+  if (warp == 12) {
+    dev::tmem_alloc(&bar.tmem, 512);
+    dev::tmem_relinquish();
+  }
+  dev::tc_fence_before();
+  __syncthreads();
+  dev::tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DIM};
+  auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+    if (bar.abort) return false;
+    if (dev::mbar_wait(b, parity, err)) return true;
+    bar.abort = 1;
+    return false;
+  };
+
+  if (warp >= 12) {
+    // ---------------------------------------------------------------- MMA issuer
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 12 && lane == 0 && ntiles > 0) {
+      constexpr uint32_t idS = dev::umma_idesc(1, 0, 0, 0, 0, 128, kKeys), idO = dev::umma_idesc(1, 0, 0, 0, 1, 128, DIM);
+      const uint32_t base = dev::smem_u32(smem);
+      const uint64_t dQ = dev::umma_sdesc(base + L::kQ, 16, 1024, dev::UMMA_SW128);
+      const uint64_t dK = dev::umma_sdesc(base + L::kK, 16, 1024, dev::UMMA_SW128);
+      const uint64_t dV = dev::umma_sdesc(base + L::kV, kKeys * 128, 1024, dev::UMMA_SW128);
+      auto mma_s = [&](int t, int j) {  // S of tile t against key tile j
+#pragma unroll
+        for (int ks = 0; ks < DIM / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * (kKeys * 128) + (ks & 3) * 32;
+          dev::umma<dev::MmaKind::F16>(tS[t], dQ + ((t * L::kQTile + off) >> 4), dK + (((j & 1) * L::kTile + off) >> 4), idS,
+                                       ks != 0);
+        }
+      };
+      auto mma_o = [&](int t, int j) {
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          umma_ts_f16(tO[t], tS[t] + ks * 8, dV + (((j & 1) * L::kTile + ks * 2048) >> 4), idO, (j | ks) != 0);
+      };
+      bool ok = wait(&bar.q_full, 0) && wait(&bar.k_full[0], 0);
+      dev::tc_fence_after();
+      if (ok) {
+        mma_s(0, 0);
+        dev::umma_commit(&bar.s_full[0]);
+        if (two) {
+          mma_s(1, 0);
+          dev::umma_commit(&bar.s_full[1]);
+        }
+        dev::umma_commit(&bar.k_empty[0]);
+      }
+      for (int j = 0; j < ntiles && ok; ++j) {
+        const uint32_t ph = j & 1, next = j + 1, sph = (j >> 1) & 1, nph = (next >> 1) & 1;
+        const bool more = (int)next < ntiles;
+        ok = wait(&bar.v_full[j & 1], sph) && wait(&bar.p_full[0], ph);
+        if (!ok) break;
+        dev::tc_fence_after();
+        mma_o(0, j);
+        if (!two) dev::umma_commit(&bar.v_empty[j & 1]);
+        if (more) {
+          if (!(ok = wait(&bar.k_full[next & 1], nph))) break;
+          dev::tc_fence_after();
+          mma_s(0, next);
+          dev::umma_commit(&bar.s_full[0]);
+          if (!two) dev::umma_commit(&bar.k_empty[next & 1]);
+        }
+        if (two) {
+          if (!(ok = wait(&bar.p_full[1], ph))) break;
+          dev::tc_fence_after();
+          mma_o(1, j);
+          dev::umma_commit(&bar.v_empty[j & 1]);
+          if (more) {
+            mma_s(1, next);
+            dev::umma_commit(&bar.s_full[1]);
+            dev::umma_commit(&bar.k_empty[next & 1]);
+          }
+        }
+      }
+      if (ok) {
+        dev::umma_commit(&bar.o_full);
+      } else {
+        bar.abort = 1;
+        dev::umma_commit(&bar.drain);
+        dev::mbar_wait(&bar.drain, 0, nullptr, 200000000ull);
+      }
+    }
+  } else if (warp >= 8) {
+    // ---------------------------------------------------------------- converters
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+    constexpr int N = DIM / 16;  // 16-code loads per thread, tile and operand
+    const int cw = warp - 8, ct = threadIdx.x - 256;
+    const int lg = a.kv.page_log2;
+    // Lanes take 4 chunks x 8 rows at a time: 64-byte segments from memory and, as neighbouring
+    // rows swizzle to the other parity of 16-byte units, shared-memory stores without conflicts.
+    // Load i: rows cw * 32 + (i / (DIM / 64)) * 8 + lane / 4, chunk (i % (DIM / 64)) * 4 + lane % 4.
+    int pid[2], pid_next[2];
+    float2 sc = {0.f, 0.f};
+    int sc_ok = 0;
+    // page of the 16 keys from `key` on; -1 where no row of the block sees them, or it is out of
+    // range (reported)
+    auto page_of = [&](int key) -> int {
+      return key < kr.hi && key + 15 >= kr.lo ? seq_page(a.b, seq, key >> lg, a.kv.pages, err) : -1;
+    };
+    auto load_pids = [&](int j, int (&o)[2]) {
+      const int key = (tile0 + j) * kKeys + cw * 32;
+      o[0] = page_of(key);
+      o[1] = page_of(key + 16);
+    };
+    auto load_scales = [&](int j) {
+      if (ct < kUnits) {
+        const int pg = page_of((tile0 + j) * kKeys + ct * 16);
+        sc_ok = pg >= 0;
+        if (sc_ok) {
+          const size_t at = (size_t)pg * a.kv.heads + head;
+          sc = make_float2(a.kv.ks[at], a.kv.vs[at]);
+        }
+      }
+    };
+    auto load_tile = [&](const int8_t* codes, int j, const int (&pg)[2], uint4 (&r)[N]) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = cw * 32 + (i / L::kChunks) * 8 + (lane >> 2), c = (i % L::kChunks) * 4 + (lane & 3);
+        const int pgi = pg[(i / L::kChunks) >> 1];
+        const int slot = row & (a.kv.page - 1);  // tiles start at multiples of every page size
+        r[i] = make_uint4(0x0, 0x0, 0x0, 0x0);
+        if (pgi >= 0)
+          r[i] = __ldg(reinterpret_cast<const uint4*>(codes + (((size_t)pgi * a.kv.heads + head) * a.kv.page + slot) * DIM + c * 16));
+      }
+    };
+    auto put_tile = [&](uint8_t* tile, const uint4 (&r)[N]) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        put_codes(tile, cw * 32 + (i / L::kChunks) * 8 + (lane >> 2), (i % L::kChunks) * 4 + (lane & 3), r[i]);
+    };
+    uint4 kreg[N], vreg[N];
+    if (ntiles > 0) {
+      load_pids(0, pid);
+      load_scales(0);
+      load_tile(a.kv.k, 0, pid, kreg);
+      load_tile(a.kv.v, 0, pid, vreg);
+      if (ntiles > 1) load_pids(1, pid_next);
+    }
+    for (int j = 0; j < ntiles; ++j) {
+      const int st = j & 1;
+      const uint32_t eph = ((j >> 1) & 1) ^ 1;
+      const bool more = j + 1 < ntiles;
+      if (!wait(&bar.k_empty[st], eph)) break;
+      put_tile(smem + L::kK + st * L::kTile, kreg);
+      if (ct < kUnits) {
+        // a missing page's keys are masked (past the length) or not seen (out of range)
+        const float vs = fmaxf(sc.y, 0x1p-100f);
+        scales[(j % kScaleRing) * kUnits + ct] =
+            sc_ok ? make_float4(fabsf(a.scale) * sc.x * 1.4426950408889634f, log2f(vs), 1.0f / vs, 0.0f)
+                  : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+      }
+      dev::fence_proxy_async_smem();
+      dev::mbar_arrive(&bar.k_full[st]);
+      if (more) {
+        load_scales(j + 1);
+        load_tile(a.kv.k, j + 1, pid_next, kreg);
+      }
+      if (!wait(&bar.v_empty[st], eph)) break;
+      put_tile(smem + L::kV + st * L::kTile, vreg);
+      dev::fence_proxy_async_smem();
+      dev::mbar_arrive(&bar.v_full[st]);
+      if (more) {
+        load_tile(a.kv.v, j + 1, pid_next, vreg);
+        if (j + 2 < ntiles) load_pids(j + 2, pid_next);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax, one row per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    const int t = warp >> 2, row = threadIdx.x & 127;
+    const int r = r0 + t * 128 + row;
+    const bool in = r < rows;
+    const int tok = r / a.group, hq = head * a.group + r - tok * a.group;
+    float q_unit = 1.0f;
+    {
+      // the row to shared memory as fp16, scaled by a power of two
+      const T* src = static_cast<const T*>(a.q) + (long long)(sv.row0 + tok) * a.q_token + (long long)hq * a.q_head;
+      const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+      float top = 0.0f;
+      if (in) {
+#pragma unroll 4
+        for (int d = 0; d < DIM; d += 8) {
+          float x[8];
+          load8(src + d, vec, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        }
+      }
+      int ex = 0;
+      if (top > 0.0f && top <= 3.4028234663852886e38f) frexpf(top, &ex);
+      ex = min(max(ex, -100), 126);
+      const float down = copysignf(exp2f((float)-ex), a.scale);
+      q_unit = exp2f((float)ex);
+      uint8_t* tile = smem + L::kQ + t * L::kQTile + row * 128;
+#pragma unroll 4
+      for (int d = 0; d < DIM; d += 8) {
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (in) load8(src + d, vec, x);
+        uint4 o;
+        o.x = pack_f16(x[0] * down, x[1] * down), o.y = pack_f16(x[2] * down, x[3] * down);
+        o.z = pack_f16(x[4] * down, x[5] * down), o.w = pack_f16(x[6] * down, x[7] * down);
+        *reinterpret_cast<uint4*>(tile + (d >> 6) * (128 * 128) + ((((d >> 3) & 7) ^ (row & 7)) << 4)) = o;
+      }
+      dev::fence_proxy_async_smem();
+      dev::mbar_arrive(&bar.q_full);
+    }
+    const int pos = sv.len - sv.n + tok;
+    const int see_hi = !in || pos < 0 ? 0 : a.causal ? min(sv.len, pos + 1) : sv.len;
+    const int see_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    const bool active = t == 0 || two;
+    for (int j = 0; j < ntiles && active; ++j) {
+      if (!(ok = wait(&bar.s_full[t], j & 1))) break;
+      dev::tc_fence_after();
+      float s[kKeys];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld32p(tS[t] + lanes + i * 32, s + 32 * i);
+      dev::tmem_ld_wait();
+      const float4* sc = scales + (j % kScaleRing) * kUnits;
+      const int k0 = (tile0 + j) * kKeys;
+      const int lo = see_lo - k0, hi = see_hi - k0;
+      if (__any_sync(0xffffffffu, lo > 0 || hi < kKeys)) {
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i)
+          if (i < lo || i >= hi) s[i] = -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        float x = s[16 * u];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) x = fmaxf(x, s[16 * u + i]);
+        const float4 f = sc[u];
+        top = fmaxf(top, fmaf(x, fmaxf(f.x * q_unit, kLeast), f.y));
+      }
+      float b = 1.0f;
+      const bool move = __any_sync(0xffffffffu, top > m + kMost);
+      if (move) {
+        const float n = fmaxf(m, top - kTop);
+        b = m == n ? 1.0f : ex2(m - n);
+        m = n;
+        l *= b;
+      }
+      const float m0 = m == -INFINITY ? 0.0f : m;
+      uint32_t w[kKeys / 2];
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const float4 f = sc[u];
+        const float fx = fmaxf(f.x * q_unit, kLeast), off = f.y - m0;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float e0 = ex2(fmaf(s[16 * u + i], fx, off)), e1 = ex2(fmaf(s[16 * u + i + 1], fx, off));
+          sum += e0 + e1;
+          w[8 * u + i / 2] = pack_f16(e0, e1);
+        }
+        l = fmaf(sum, f.z, l);
+      }
+      tmem_st32(tS[t] + lanes, w);
+      tmem_st32(tS[t] + lanes + 32, w + 32);
+      if (move && j > 0) {  // S of tile j was issued after O's product of tile j - 1, which is done
+#pragma unroll 1
+        for (int i = 0; i < DIM / 32; ++i) {
+          float o[32];
+          tmem_ld32p(tO[t] + lanes + i * 32, o);
+          dev::tmem_ld_wait();
+          uint32_t x[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(o[e] * b);
+          tmem_st32(tO[t] + lanes + i * 32, x);
+        }
+      }
+      tmem_st_wait();
+      dev::tc_fence_before();
+      dev::mbar_arrive(&bar.p_full[t]);
+    }
+    if (ok && ntiles > 0) ok = wait(&bar.o_full, 0);
+    dev::tc_fence_after();
+    if (active) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const bool whole = nsplit == 1;
+      T* dst = static_cast<T*>(a.out) + (long long)(sv.row0 + tok) * a.o_token + (long long)hq * a.o_head;
+      const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+      const size_t at = ((size_t)(sv.row0 + tok) * a.q_heads + hq) * p.splits + part;
+#pragma unroll 1
+      for (int i = 0; i < DIM / 32; ++i) {
+        float o[32];
+        if (ntiles > 0) {
+          tmem_ld32p(tO[t] + lanes + i * 32, o);
+          dev::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+        }
+        if (!in || !ok) continue;
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = l == 0.0f ? 0.0f : o[e + k] * inv;
+            store8(dst + i * 32 + e, vec, x);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(p.part_o + at * DIM + i * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      if (in && ok) {
+        if (!whole)
+          p.part_ml[at] = make_float2(m, l);
+        else if (a.lse)
+          a.lse[(long long)(sv.row0 + tok) * a.q_heads + hq] =
+              l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+      }
+    }
+  }
+  dev::tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    dev::tc_fence_after();
+    dev::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the key parts of split rows, in the order of the parts: one warp per (token, head).
+template <typename T, int DIM>
+__global__ void __launch_bounds__(128) k_attn_join(const TcArgs p, unsigned* err) {
+  const AttnArgs& a = p.a;
+  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, seq = blockIdx.y;
+  const SeqView sv = seq_view(a.b, seq, err);
+  if (item >= (long long)sv.n * a.q_heads) return;
+  const int tok = (int)(item / a.q_heads), hq = (int)(item - (long long)tok * a.q_heads);
+  const int r = tok * a.group + hq % a.group, r0 = r / kRows * kRows;
+  const KeyRange kr = key_range(a, sv, r0, min(kRows, sv.n * a.group - r0), kKeys);
+  const int nsplit = max(1, (kr.n + p.chunk - 1) / p.chunk);
+  if (nsplit == 1) return;  // written whole
+  const size_t at = ((size_t)(sv.row0 + tok) * a.q_heads + hq) * p.splits;
+  float top = -INFINITY, sum = 0.0f;
+  for (int k = 0; k < nsplit; ++k) top = fmaxf(top, p.part_ml[at + k].x);
+  float o[DIM / 32] = {};
+  for (int k = 0; k < nsplit; ++k) {
+    const float2 ml = p.part_ml[at + k];
+    const float b = ml.x == top ? 1.0f : ex2(ml.x - top);
+    sum = fmaf(ml.y, b, sum);
+#pragma unroll
+    for (int i = 0; i < DIM / 32; ++i) o[i] = fmaf(p.part_o[(at + k) * DIM + i * 32 + lane], b, o[i]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T* dst = static_cast<T*>(a.out) + (long long)(sv.row0 + tok) * a.o_token + (long long)hq * a.o_head;
+#pragma unroll
+  for (int i = 0; i < DIM / 32; ++i) dst[i * 32 + lane] = from_f<T>(sum == 0.0f ? 0.0f : o[i] * inv);
+  if (lane == 0 && a.lse)
+    a.lse[(long long)(sv.row0 + tok) * a.q_heads + hq] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+}
+
+template <typename T, int DIM>
+bool tc_launch(Call& c, const AttnArgs& a) {
+  using L = TcSmem<DIM>;
+  static bool attr_done[64] = {false};
+  const int dv = current_device() & 63;
+  if (!attr_done[dv]) {
+    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_tc<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes)))
+      return false;
+    attr_done[dv] = true;
+  }
+  TcArgs p = {};
+  p.a = a;
+  const long long max_new = std::min(a.b.max_new, a.b.tokens);
+  p.row_tiles = (int)((max_new * a.group + kRows - 1) / kRows);
+  // few blocks: the keys are split so that every SM gets one, in parts of at least 4 key tiles
+  const long long work = (long long)p.row_tiles * a.kv.heads * a.b.seqs;
+  const int tiles = (a.b.max_len + kKeys - 1) / kKeys + 1;  // a window can start inside a tile
+  const long long want = std::max<long long>(1, c.sm_count() / std::max<long long>(1, work));
+  p.chunk = (int)std::max<long long>(4, (tiles + want - 1) / want);
+  p.splits = (tiles + p.chunk - 1) / p.chunk;
+  if (p.splits > 1) {
+    const size_t n = (size_t)a.b.tokens * a.q_heads * p.splits;
+    p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
+    p.part_ml = (float2*)c.scratch(n * sizeof(float2));
+    if (!c.ok()) return false;
+  }
+  k_attn_tc<T, DIM><<<dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), kTcThreads, L::kBytes, c.stream()>>>(p, c.err());
+  if (!c.launched("k_attn_tc")) return false;
+  if (p.splits > 1) {
+    const long long items = (max_new * a.q_heads + 3) / 4;
+    k_attn_join<T, DIM><<<dim3((unsigned)items, a.b.seqs), 128, 0, c.stream()>>>(p, c.err());
+    return c.launched("k_attn_join");
+  }
+  return true;
+}
+
+}  // namespace
+
+bool attn_tc_dev(Call& c, const AttnArgs& a) {
+  if (a.dtype == ACFUN_F16) return a.kv.dim == 64 ? tc_launch<__half, 64>(c, a) : tc_launch<__half, 128>(c, a);
+  return a.kv.dim == 64 ? tc_launch<__nv_bfloat16, 64>(c, a) : tc_launch<__nv_bfloat16, 128>(c, a);
+}
+
+bool attn_tc_takes(const AttnArgs& a) {
+  const long long rows = (long long)std::min(a.b.max_new, a.b.tokens) * a.group;
+  return (a.kv.dim == 64 || a.kv.dim == 128) && rows > 64 && rows * a.kv.heads < (1LL << 31);
+}
+
+}  // namespace acf
