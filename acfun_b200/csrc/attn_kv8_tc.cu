@@ -98,19 +98,43 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 16 codes to fp16, written as two 16-byte units of row `row` of a swizzled operand tile: code
-// chunk c (16 codes) of the row lies in column chunk c / 4.
-__device__ __forceinline__ void put_codes(uint8_t* tile, int row, int c, uint4 w) {
-  const uint32_t in[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-  uint8_t* base = tile + (c >> 2) * (kKeys * 128) + row * 128;
-  const int u = 2 * (c & 3), x = row & 7;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint4 o;
-    o.x = f16_from_u8(in[2 * h], 0x4140), o.y = f16_from_u8(in[2 * h], 0x4342);
-    o.z = f16_from_u8(in[2 * h + 1], 0x4140), o.w = f16_from_u8(in[2 * h + 1], 0x4342);
-    *reinterpret_cast<uint4*>(base + (((u + h) ^ x) << 4)) = o;
-  }
+__device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(t)
+      : "memory");
+}
+// Two 32-bit operations per instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Eight codes (already XORed with 0x80 each) to fp16, one 16-byte unit.
+__device__ __forceinline__ void put8(uint8_t* p, uint32_t w0, uint32_t w1) {
+  uint4 o;
+  o.x = f16_from_u8(w0, 0x4140), o.y = f16_from_u8(w0, 0x4342);
+  o.z = f16_from_u8(w1, 0x4140), o.w = f16_from_u8(w1, 0x4342);
+  *reinterpret_cast<uint4*>(p) = o;
 }
 
 template <typename T, int DIM>
@@ -136,14 +160,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
   const bool two = nr > 128;
 
   if (threadIdx.x == 0) {
-    dev::mbar_init(&bar.q_full, 256);
+    dev::mbar_init(&bar.q_full, 8);
     for (int i = 0; i < 2; ++i) {
-      dev::mbar_init(&bar.k_full[i], 128);
+      dev::mbar_init(&bar.k_full[i], 4);
       dev::mbar_init(&bar.k_empty[i], 1);
-      dev::mbar_init(&bar.v_full[i], 128);
+      dev::mbar_init(&bar.v_full[i], 4);
       dev::mbar_init(&bar.v_empty[i], 1);
       dev::mbar_init(&bar.s_full[i], 1);
-      dev::mbar_init(&bar.p_full[i], 128);
+      dev::mbar_init(&bar.p_full[i], 4);
     }
     dev::mbar_init(&bar.o_full, 1);
     dev::mbar_init(&bar.drain, 1);
@@ -158,35 +182,50 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
   __syncthreads();
   dev::tc_fence_after();
   const uint32_t tmem = bar.tmem;
-  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DIM};
+  const uint32_t tS0 = tmem, tO0 = tmem + 256;  // tile t: S at tS0 + 128 t, O at tO0 + DIM t
   auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+    if (dev::mbar_try_wait(dev::smem_u32(b), parity)) return true;
     if (bar.abort) return false;
     if (dev::mbar_wait(b, parity, err)) return true;
     bar.abort = 1;
     return false;
   };
+  // one arrival for the warp, after what its lanes did
+  auto arrive = [&](uint64_t* b) {
+    __syncwarp();
+    if (lane == 0) dev::mbar_arrive(b);
+  };
 
   if (warp >= 12) {
     // ---------------------------------------------------------------- MMA issuer
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 12 && lane == 0 && ntiles > 0) {
       constexpr uint32_t idS = dev::umma_idesc(1, 0, 0, 0, 0, 128, kKeys), idO = dev::umma_idesc(1, 0, 0, 0, 1, 128, DIM);
       const uint32_t base = dev::smem_u32(smem);
       const uint64_t dQ = dev::umma_sdesc(base + L::kQ, 16, 1024, dev::UMMA_SW128);
       const uint64_t dK = dev::umma_sdesc(base + L::kK, 16, 1024, dev::UMMA_SW128);
       const uint64_t dV = dev::umma_sdesc(base + L::kV, kKeys * 128, 1024, dev::UMMA_SW128);
+      // Descriptors are formed anew for each group of products: left to itself the compiler keeps all
+      // of them across the loop, which in this role's registers means local memory, and a load from it
+      // per instruction made the products of S four times as long as the tensor cores take.
+      auto fresh = [](uint64_t d) {
+        uint64_t r;
+        asm volatile("mov.b64 %0, %1;" : "=l"(r) : "l"(d));
+        return r;
+      };
       auto mma_s = [&](int t, int j) {  // S of tile t against key tile j
+        const uint64_t q = fresh(dQ + ((t * L::kQTile) >> 4)), k = fresh(dK + (((j & 1) * L::kTile) >> 4));
 #pragma unroll
         for (int ks = 0; ks < DIM / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (kKeys * 128) + (ks & 3) * 32;
-          dev::umma<dev::MmaKind::F16>(tS[t], dQ + ((t * L::kQTile + off) >> 4), dK + (((j & 1) * L::kTile + off) >> 4), idS,
-                                       ks != 0);
+          const uint32_t off = ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32) >> 4;
+          dev::umma<dev::MmaKind::F16>(tS0 + t * 128, q + off, k + off, idS, ks != 0);
         }
       };
       auto mma_o = [&](int t, int j) {
+        const uint64_t v = fresh(dV + (((j & 1) * L::kTile) >> 4));
 #pragma unroll
         for (int ks = 0; ks < kKeys / 16; ++ks)
-          umma_ts_f16(tO[t], tS[t] + ks * 8, dV + (((j & 1) * L::kTile + ks * 2048) >> 4), idO, (j | ks) != 0);
+          umma_ts_f16(tO0 + t * DIM, tS0 + t * 128 + ks * 8, v + ((ks * 2048) >> 4), idO, (j | ks) != 0);
       };
       bool ok = wait(&bar.q_full, 0) && wait(&bar.k_full[0], 0);
       dev::tc_fence_after();
@@ -243,22 +282,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
     // Lanes take 4 chunks x 8 rows at a time: 64-byte segments from memory and, as neighbouring
     // rows swizzle to the other parity of 16-byte units, shared-memory stores without conflicts.
     // Load i: rows cw * 32 + (i / (DIM / 64)) * 8 + lane / 4, chunk (i % (DIM / 64)) * 4 + lane % 4.
-    int pid[2], pid_next[2];
+    // Page numbers are fetched two tiles ahead of their use and looked at only then: a check right
+    // after the load would wait for memory twice per tile.
+    int next_pid[2], next_sc = -1;
     float2 sc = {0.f, 0.f};
     int sc_ok = 0;
-    // page of the 16 keys from `key` on; -1 where no row of the block sees them, or it is out of
-    // range (reported)
-    auto page_of = [&](int key) -> int {
-      return key < kr.hi && key + 15 >= kr.lo ? seq_page(a.b, seq, key >> lg, a.kv.pages, err) : -1;
+    // page of the 16 keys from `key` on; -1 where no row of the block sees them
+    auto fetch_pid = [&](int key) -> int {
+      return key < kr.hi && key + 15 >= kr.lo ? __ldg(a.b.table + (size_t)seq * a.b.cols + (key >> lg)) : -1;
     };
-    auto load_pids = [&](int j, int (&o)[2]) {
-      const int key = (tile0 + j) * kKeys + cw * 32;
-      o[0] = page_of(key);
-      o[1] = page_of(key + 16);
+    // a page number that is out of range is reported, and its keys are not seen
+    auto good = [&](int pid, int key) -> int {
+      if ((unsigned)pid < (unsigned)a.kv.pages) return pid;
+      if (key < kr.hi && key + 15 >= kr.lo) atomicOr(err, ACF_DEV_ERR_BADARG);
+      return -1;
     };
-    auto load_scales = [&](int j) {
+    auto fetch = [&](int j) {
+      const int key = (tile0 + j) * kKeys;
+      next_pid[0] = fetch_pid(key + cw * 32);
+      next_pid[1] = fetch_pid(key + cw * 32 + 16);
+      if (ct < kUnits) next_sc = fetch_pid(key + ct * 16);
+    };
+    int pid[2];
+    auto take = [&](int j) {  // the fetched numbers become tile j's; its scales are requested
+      const int key = (tile0 + j) * kKeys;
+      pid[0] = good(next_pid[0], key + cw * 32);
+      pid[1] = good(next_pid[1], key + cw * 32 + 16);
       if (ct < kUnits) {
-        const int pg = page_of((tile0 + j) * kKeys + ct * 16);
+        const int pg = good(next_sc, key + ct * 16);
         sc_ok = pg >= 0;
         if (sc_ok) {
           const size_t at = (size_t)pg * a.kv.heads + head;
@@ -266,29 +317,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
         }
       }
     };
-    auto load_tile = [&](const int8_t* codes, int j, const int (&pg)[2], uint4 (&r)[N]) {
+    const int key_in_unit = lane >> 2;
+    auto load_tile = [&](const int8_t* codes, uint4 (&r)[N]) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int row = cw * 32 + (i / L::kChunks) * 8 + (lane >> 2), c = (i % L::kChunks) * 4 + (lane & 3);
-        const int pgi = pg[(i / L::kChunks) >> 1];
-        const int slot = row & (a.kv.page - 1);  // tiles start at multiples of every page size
-        r[i] = make_uint4(0x0, 0x0, 0x0, 0x0);
-        if (pgi >= 0)
-          r[i] = __ldg(reinterpret_cast<const uint4*>(codes + (((size_t)pgi * a.kv.heads + head) * a.kv.page + slot) * DIM + c * 16));
+      for (int u = 0; u < 2; ++u) {
+        const int slot = (cw * 32 + u * 16 + key_in_unit) & (a.kv.page - 1);  // tiles start at multiples of every page size
+        const int8_t* src = codes + (((size_t)max(pid[u], 0) * a.kv.heads + head) * a.kv.page + slot) * DIM + (lane & 3) * 16;
+#pragma unroll
+        for (int i = u * N / 2; i < (u + 1) * N / 2; ++i) {
+          r[i] = make_uint4(0, 0, 0, 0);
+          if (pid[u] >= 0)
+            r[i] = __ldg(reinterpret_cast<const uint4*>(src + ((i / L::kChunks) & 1) * 8 * DIM + (i % L::kChunks) * 64));
+        }
       }
     };
+    // this thread's two 16-byte units of row cw * 32 + lane / 4; its other rows are 8 apart
+    const int unit0 = (cw * 32 + key_in_unit) * 128 + (((2 * (lane & 3)) ^ key_in_unit) << 4);
+    const int unit1 = (cw * 32 + key_in_unit) * 128 + (((2 * (lane & 3) + 1) ^ key_in_unit) << 4);
     auto put_tile = [&](uint8_t* tile, const uint4 (&r)[N]) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        put_codes(tile, cw * 32 + (i / L::kChunks) * 8 + (lane >> 2), (i % L::kChunks) * 4 + (lane & 3), r[i]);
+      for (int i = 0; i < N; ++i) {
+        const int off = (i / L::kChunks) * 8 * 128 + (i % L::kChunks) * (kKeys * 128);
+        put8(tile + unit0 + off, r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u);
+        put8(tile + unit1 + off, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u);
+      }
     };
     uint4 kreg[N], vreg[N];
     if (ntiles > 0) {
-      load_pids(0, pid);
-      load_scales(0);
-      load_tile(a.kv.k, 0, pid, kreg);
-      load_tile(a.kv.v, 0, pid, vreg);
-      if (ntiles > 1) load_pids(1, pid_next);
+      fetch(0);
+      take(0);
+      if (ntiles > 1) fetch(1);
+      load_tile(a.kv.k, kreg);
+      load_tile(a.kv.v, vreg);
     }
     for (int j = 0; j < ntiles; ++j) {
       const int st = j & 1;
@@ -304,23 +364,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
                   : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
       }
       dev::fence_proxy_async_smem();
-      dev::mbar_arrive(&bar.k_full[st]);
+      arrive(&bar.k_full[st]);
       if (more) {
-        load_scales(j + 1);
-        load_tile(a.kv.k, j + 1, pid_next, kreg);
+        take(j + 1);
+        if (j + 2 < ntiles) fetch(j + 2);
+        load_tile(a.kv.k, kreg);
       }
       if (!wait(&bar.v_empty[st], eph)) break;
       put_tile(smem + L::kV + st * L::kTile, vreg);
       dev::fence_proxy_async_smem();
-      dev::mbar_arrive(&bar.v_full[st]);
-      if (more) {
-        load_tile(a.kv.v, j + 1, pid_next, vreg);
-        if (j + 2 < ntiles) load_pids(j + 2, pid_next);
-      }
+      arrive(&bar.v_full[st]);
+      if (more) load_tile(a.kv.v, vreg);
     }
   } else {
     // ---------------------------------------------------------------- softmax, one row per thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = warp >> 2, row = threadIdx.x & 127;
     const int r = r0 + t * 128 + row;
     const bool in = r < rows;
@@ -356,7 +414,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
         *reinterpret_cast<uint4*>(tile + (d >> 6) * (128 * 128) + ((((d >> 3) & 7) ^ (row & 7)) << 4)) = o;
       }
       dev::fence_proxy_async_smem();
-      dev::mbar_arrive(&bar.q_full);
+      arrive(&bar.q_full);
     }
     const int pos = sv.len - sv.n + tok;
     const int see_hi = !in || pos < 0 ? 0 : a.causal ? min(sv.len, pos + 1) : sv.len;
@@ -370,22 +428,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
       dev::tc_fence_after();
       float s[kKeys];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32p(tS[t] + lanes + i * 32, s + 32 * i);
+      for (int i = 0; i < 4; ++i) tmem_ld32p(tS0 + t * 128 + lanes + i * 32, s + 32 * i);
       dev::tmem_ld_wait();
       const float4* sc = scales + (j % kScaleRing) * kUnits;
       const int k0 = (tile0 + j) * kKeys;
       const int lo = see_lo - k0, hi = see_hi - k0;
       if (__any_sync(0xffffffffu, lo > 0 || hi < kKeys)) {
+        // opaque bounds: the comparisons stay inside this branch instead of running for every tile
+        int from = lo, to = hi;
+        asm volatile("" : "+r"(from), "+r"(to));
 #pragma unroll
         for (int i = 0; i < kKeys; ++i)
-          if (i < lo || i >= hi) s[i] = -INFINITY;
+          if (i < from || i >= to) s[i] = -INFINITY;
       }
       float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        float x = s[16 * u];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) x = fmaxf(x, s[16 * u + i]);
+        const float* v = s + 16 * u;
+        const float x0 = max3(max3(v[0], v[1], v[2]), v[3], v[4]), x1 = max3(max3(v[5], v[6], v[7]), v[8], v[9]);
+        const float x2 = max3(max3(v[10], v[11], v[12]), v[13], v[14]);
+        const float x = max3(fmaxf(x0, v[15]), x1, x2);
         const float4 f = sc[u];
         top = fmaxf(top, fmaf(x, fmaxf(f.x * q_unit, kLeast), f.y));
       }
@@ -398,37 +460,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
         l *= b;
       }
       const float m0 = m == -INFINITY ? 0.0f : m;
-      uint32_t w[kKeys / 2];
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const float4 f = sc[u];
-        const float fx = fmaxf(f.x * q_unit, kLeast), off = f.y - m0;
-        float sum = 0.0f;
+      for (int h = 0; h < 4; ++h) {  // 32 keys: 16 registers of weights
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float e0 = ex2(fmaf(s[16 * u + i], fx, off)), e1 = ex2(fmaf(s[16 * u + i + 1], fx, off));
-          sum += e0 + e1;
-          w[8 * u + i / 2] = pack_f16(e0, e1);
+        for (int v = 0; v < 2; ++v) {
+          const int u = 2 * h + v;
+          const float4 f = sc[u];
+          const float fx = fmaxf(f.x * q_unit, kLeast), off = f.y - m0;
+          const float2 fx2 = make_float2(fx, fx), off2 = make_float2(off, off);
+          float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float2 e = fma2(make_float2(s[16 * u + i], s[16 * u + i + 1]), fx2, off2);
+            e.x = ex2(e.x), e.y = ex2(e.y);
+            sum = add2(sum, e);
+            w[8 * v + i / 2] = pack_f16(e.x, e.y);
+          }
+          l = fmaf(sum.x + sum.y, f.z, l);
         }
-        l = fmaf(sum, f.z, l);
+        tmem_st16(tS0 + t * 128 + lanes + 16 * h, w);
       }
-      tmem_st32(tS[t] + lanes, w);
-      tmem_st32(tS[t] + lanes + 32, w + 32);
       if (move && j > 0) {  // S of tile j was issued after O's product of tile j - 1, which is done
 #pragma unroll 1
         for (int i = 0; i < DIM / 32; ++i) {
           float o[32];
-          tmem_ld32p(tO[t] + lanes + i * 32, o);
+          tmem_ld32p(tO0 + t * DIM + lanes + i * 32, o);
           dev::tmem_ld_wait();
           uint32_t x[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(o[e] * b);
-          tmem_st32(tO[t] + lanes + i * 32, x);
+          tmem_st32(tO0 + t * DIM + lanes + i * 32, x);
         }
       }
       tmem_st_wait();
       dev::tc_fence_before();
-      dev::mbar_arrive(&bar.p_full[t]);
+      arrive(&bar.p_full[t]);
     }
     if (ok && ntiles > 0) ok = wait(&bar.o_full, 0);
     dev::tc_fence_after();
@@ -442,7 +509,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
       for (int i = 0; i < DIM / 32; ++i) {
         float o[32];
         if (ntiles > 0) {
-          tmem_ld32p(tO[t] + lanes + i * 32, o);
+          tmem_ld32p(tO0 + t * DIM + lanes + i * 32, o);
           dev::tmem_ld_wait();
         } else {
 #pragma unroll
