@@ -156,11 +156,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
           for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to_f(src[(i / 4) * 64 + c * 16 + 4 * (i % 4) + e])));
       }
       top = quad_max(top);
-      int ex = 0;
-      if (top > 0.0f && top <= 3.4028234663852886e38f) frexpf(top, &ex);
-      ex = min(max(ex, -100), 126);
-      const float down = exp2f((float)-ex);
-      q_unit[rr] = exp2f((float)ex);
+      const Pow2 f = row_pow2(top);
+      const float down = f.down;
+      q_unit[rr] = f.up;
 #pragma unroll
       for (int i = 0; i < DIM / 16; ++i) {
         float x[4];

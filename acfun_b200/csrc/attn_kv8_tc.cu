@@ -12,9 +12,12 @@
 //
 //   warps 0-3, 4-7  Q of tile A / B to shared memory, then its softmax and output (a TMEM lane and
 //                   a row per thread)
-//   warps 8-11      codes from global memory, one tile ahead in registers, to fp16 in the 128-byte
-//                   swizzled layout of the MMA operands; two stages each for K and V
-//   warp 12         the MMA issuer; warps 13-15 only lend their registers
+// The codes become fp16 in the 128-byte swizzled layout of the MMA operands in one of two places:
+//   in the kernel   warps 8-11 convert the block's keys one tile ahead (two stages each for K and V),
+//                   warp 12 issues the MMAs; the cache is read once per 256 rows, at one byte a code
+//   before it       k_kv8_tiles writes each key tile's image to scratch once, and warp 9 only copies
+//                   images (cp.async.bulk), warp 8 issues the MMAs.  Conversion costs the softmax's
+//                   issue slots and registers, and with many row tiles it is repeated for each.
 // TMEM: S of A and B (128 columns each; the fp16 weights overlay their first half), O of A and B.
 // Every wait is bounded (ptx.cuh); on expiry the error word is set and all roles leave.
 #include <math.h>
@@ -26,11 +29,25 @@
 namespace acf {
 namespace {
 
-constexpr int kTcThreads = 512;
+// Threads, and the registers (per thread) of the softmax warps, of the converters, and of the warps that
+// issue; per warpgroup their sum is what the block is launched with.
+template <bool PRE>
+struct Roles;
+template <>
+struct Roles<false> {
+  static constexpr int kThreads = 512, kMmaWarp = 12;  // 2 x 168 + 112 + 64 = 4 x 128
+};
+template <>
+struct Roles<true> {
+  static constexpr int kThreads = 384, kMmaWarp = 8, kCopyWarp = 9;  // 2 x 216 + 72 = 3 x 168
+};
 constexpr int kRows = 256;     // packed rows of a block
 constexpr int kKeys = 128;     // keys per step
 constexpr int kUnits = kKeys / 16;
+constexpr int kFmaOf4 = 1;      // pairs of four whose 2^x the FMA units compute instead of the special function unit
 constexpr float kLeast = 1e-37f;  // a factor never underflows to 0: a masked score stays -inf under it
+constexpr int kPreRowTiles = 3;
+constexpr size_t kPreBytes = size_t(1) << 30;
 constexpr int kScaleRing = 4;  // the converters are at most two tiles ahead of a softmax
 
 struct TcArgs {
@@ -40,6 +57,11 @@ struct TcArgs {
   float* part_o;   // [tokens][q_heads][splits][DIM], null when splits == 1
   float2* part_ml;
   int row_tiles;
+  // images of the key tiles made before the kernel: [seqs][heads][tiles] of K, V and their scales
+  uint8_t* k_img;
+  uint8_t* v_img;
+  float4* scale_img;
+  int tiles;
 };
 
 template <int DIM>
@@ -55,7 +77,7 @@ struct TcSmem {
 
 struct TcBars {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_full, drain;
+  uint64_t s_full[2], p_full[2][2], o_full, drain;
   uint32_t tmem;
   volatile int abort;
 };
@@ -80,16 +102,13 @@ __device__ __forceinline__ void tmem_ld32p(uint32_t t, float* r) {
         "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(t));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16p(uint32_t t, float* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t)
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(t));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -123,6 +142,23 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// 2^x of two values with the FMA units, for x >= -126: a fourth-degree minimax polynomial of the
+// fraction (relative error 2.6e-6; one degree less would show in the sums, and so in lse) and the
+// integer part added to its exponent.
+__device__ __forceinline__ float2 ex2_fma2(float2 x) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
+  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  const float2 r = add2(x, make_float2(kMagic, kMagic));
+  const float2 n = add2(r, make_float2(-kMagic, -kMagic));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 y = fma2(f, make_float2(0.009570102f, 0.009570102f), make_float2(0.05591786f, 0.05591786f));
+  y = fma2(y, f, make_float2(0.24024744f, 0.24024744f));
+  y = fma2(y, f, make_float2(0.6931218f, 0.6931218f));
+  y = fma2(y, f, make_float2(0.9999993f, 0.9999993f));
+  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23));
+  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23));
+  return y;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -137,8 +173,66 @@ __device__ __forceinline__ void put8(uint8_t* p, uint32_t w0, uint32_t w1) {
   *reinterpret_cast<uint4*>(p) = o;
 }
 
-template <typename T, int DIM>
-__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsigned* err) {
+// What a softmax needs of 16 keys' page: factor of S, log2 and reciprocal of the V scale.  Keys of a
+// missing page are masked (past the length) or not seen (out of range): weight 0.
+__device__ __forceinline__ float4 scale_entry(float2 ks_vs, bool there, float scale) {
+  const float vs = fmaxf(ks_vs.y, 0x1p-100f);
+  return there ? make_float4(fabsf(scale) * ks_vs.x * 1.4426950408889634f, log2f(vs), 1.0f / vs, 0.0f)
+               : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+}
+
+// Images of the key tiles that some row of a sequence sees: block (tile, head, sequence), 256
+// threads, half of them for K and half for V.  Bound by the write of two bytes per code.
+template <int DIM>
+__global__ void __launch_bounds__(256) k_kv8_tiles(const TcArgs p, unsigned* err) {
+  const AttnArgs& a = p.a;
+  const int tile = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
+  const SeqView sv = seq_view(a.b, seq, err);
+  if (sv.n == 0) return;
+  const KeyRange kr = key_range(a, sv, 0, sv.n * a.group, kKeys);
+  if (tile < kr.first || tile >= kr.first + kr.n) return;
+  const int v = threadIdx.x >> 7, t = threadIdx.x & 127;
+  const int8_t* codes = v ? a.kv.v : a.kv.k;
+  const size_t at = ((size_t)seq * a.kv.heads + head) * p.tiles + tile;
+  uint8_t* img = (v ? p.v_img : p.k_img) + at * (kKeys * DIM * 2);
+  auto page_of = [&](int key) -> int {
+    return key < kr.hi && key + 15 >= kr.lo ? seq_page(a.b, seq, key >> a.kv.page_log2, a.kv.pages, err) : -1;
+  };
+  if (threadIdx.x < kUnits) {
+    const int pg = page_of(tile * kKeys + threadIdx.x * 16);
+    const size_t sc = (size_t)max(pg, 0) * a.kv.heads + head;
+    p.scale_img[at * kUnits + threadIdx.x] =
+        scale_entry(pg >= 0 ? make_float2(a.kv.ks[sc], a.kv.vs[sc]) : make_float2(0.f, 0.f), pg >= 0, a.scale);
+  }
+  constexpr int CPR = DIM / 16;  // 16-code chunks per row
+  constexpr int STEP = 128 / CPR, N = kKeys / STEP;  // rows per pass: 16 (dim 128) or 32 (dim 64); passes
+  const int c = t % CPR, r0 = t / CPR;
+  int pg[N];
+  uint4 w[N];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const int key = tile * kKeys + r * STEP + r0;
+    pg[r] = (key & ~15) < kr.hi && key + 15 >= kr.lo ? __ldg(a.b.table + (size_t)seq * a.b.cols + (key >> a.kv.page_log2)) : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const int slot = (tile * kKeys + r * STEP + r0) & (a.kv.page - 1);
+    w[r] = make_uint4(0, 0, 0, 0);
+    if ((unsigned)pg[r] < (unsigned)a.kv.pages)  // what is not is reported with the scales above
+      w[r] = __ldg(reinterpret_cast<const uint4*>(codes + (((size_t)pg[r] * a.kv.heads + head) * a.kv.page + slot) * DIM + c * 16));
+  }
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const int row = r * STEP + r0;
+    uint8_t* o = img + (c >> 2) * (kKeys * 128) + row * 128;
+    const int x = row & 7, u = 2 * (c & 3);
+    put8(o + ((u ^ x) << 4), w[r].x ^ 0x80808080u, w[r].y ^ 0x80808080u);
+    put8(o + (((u + 1) ^ x) << 4), w[r].z ^ 0x80808080u, w[r].w ^ 0x80808080u);
+  }
+}
+
+template <typename T, int DIM, bool PRE>
+__global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArgs p, unsigned* err) {
   using L = TcSmem<DIM>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -162,19 +256,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
   if (threadIdx.x == 0) {
     dev::mbar_init(&bar.q_full, 8);
     for (int i = 0; i < 2; ++i) {
-      dev::mbar_init(&bar.k_full[i], 4);
+      dev::mbar_init(&bar.k_full[i], PRE ? 1 : 4);
       dev::mbar_init(&bar.k_empty[i], 1);
-      dev::mbar_init(&bar.v_full[i], 4);
+      dev::mbar_init(&bar.v_full[i], PRE ? 1 : 4);
       dev::mbar_init(&bar.v_empty[i], 1);
       dev::mbar_init(&bar.s_full[i], 1);
-      dev::mbar_init(&bar.p_full[i], 4);
+      dev::mbar_init(&bar.p_full[i][0], 4);
+      dev::mbar_init(&bar.p_full[i][1], 4);
     }
     dev::mbar_init(&bar.o_full, 1);
     dev::mbar_init(&bar.drain, 1);
     bar.abort = 0;
     dev::fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == Roles<PRE>::kMmaWarp) {
     dev::tmem_alloc(&bar.tmem, 512);
     dev::tmem_relinquish();
   }
@@ -196,10 +291,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
     if (lane == 0) dev::mbar_arrive(b);
   };
 
-  if (warp >= 12) {
-    // ---------------------------------------------------------------- MMA issuer
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 12 && lane == 0 && ntiles > 0) {
+  if (warp >= (PRE ? 8 : 12)) {
+    // ---------------------------------------------------------------- MMA issuer, image copies
+    if constexpr (PRE)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (PRE) {
+      if (warp == Roles<PRE>::kCopyWarp && dev::elect_one()) {
+        const size_t at = ((size_t)seq * a.kv.heads + head) * p.tiles + tile0;
+        for (int j = 0; j < ntiles; ++j) {
+          const int st = j & 1;
+          const uint32_t eph = ((j >> 1) & 1) ^ 1;
+          if (!wait(&bar.k_empty[st], eph)) break;
+          dev::mbar_arrive_expect_tx(&bar.k_full[st], L::kTile + kUnits * 16);
+          dev::bulk_load(smem + L::kK + st * L::kTile, p.k_img + (at + j) * L::kTile, L::kTile, &bar.k_full[st]);
+          dev::bulk_load(scales + (j % kScaleRing) * kUnits, p.scale_img + (at + j) * kUnits, kUnits * 16, &bar.k_full[st]);
+          if (!wait(&bar.v_empty[st], eph)) break;
+          dev::mbar_arrive_expect_tx(&bar.v_full[st], L::kTile);
+          dev::bulk_load(smem + L::kV + st * L::kTile, p.v_img + (at + j) * L::kTile, L::kTile, &bar.v_full[st]);
+        }
+        // no copy may be in flight when the block leaves: the last stages' are waited for (an
+        // aborted block's too)
+        for (int j = max(0, ntiles - 2); j < ntiles; ++j) {
+          dev::mbar_wait(&bar.k_full[j & 1], (j >> 1) & 1, nullptr, 200000000ull);
+          dev::mbar_wait(&bar.v_full[j & 1], (j >> 1) & 1, nullptr, 200000000ull);
+        }
+      }
+    }
+    // The issuing thread is one that elect.sync names: with a thread picked by its lane number the
+    // compiler has to move every operand to uniform registers by itself, and next to busy softmax
+    // warps an instruction then took 116 cycles to issue instead of the 64 that it runs.
+    if (warp == Roles<PRE>::kMmaWarp && ntiles > 0 && dev::elect_one()) {
       constexpr uint32_t idS = dev::umma_idesc(1, 0, 0, 0, 0, 128, kKeys), idO = dev::umma_idesc(1, 0, 0, 0, 1, 128, DIM);
       const uint32_t base = dev::smem_u32(smem);
       const uint64_t dQ = dev::umma_sdesc(base + L::kQ, 16, 1024, dev::UMMA_SW128);
@@ -221,11 +344,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
           dev::umma<dev::MmaKind::F16>(tS0 + t * 128, q + off, k + off, idS, ks != 0);
         }
       };
-      auto mma_o = [&](int t, int j) {
+      auto mma_o = [&](int t, int j) -> bool {  // the weights of a tile come in two halves of 64 keys
         const uint64_t v = fresh(dV + (((j & 1) * L::kTile) >> 4));
 #pragma unroll
-        for (int ks = 0; ks < kKeys / 16; ++ks)
-          umma_ts_f16(tO0 + t * DIM, tS0 + t * 128 + ks * 8, v + ((ks * 2048) >> 4), idO, (j | ks) != 0);
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(&bar.p_full[t][h], j & 1)) return false;
+          dev::tc_fence_after();
+#pragma unroll
+          for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+            umma_ts_f16(tO0 + t * DIM, tS0 + t * 128 + ks * 8, v + ((ks * 2048) >> 4), idO, (j | ks) != 0);
+        }
+        return true;
       };
       bool ok = wait(&bar.q_full, 0) && wait(&bar.k_full[0], 0);
       dev::tc_fence_after();
@@ -239,24 +368,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
         dev::umma_commit(&bar.k_empty[0]);
       }
       for (int j = 0; j < ntiles && ok; ++j) {
-        const uint32_t ph = j & 1, next = j + 1, sph = (j >> 1) & 1, nph = (next >> 1) & 1;
-        const bool more = (int)next < ntiles;
-        ok = wait(&bar.v_full[j & 1], sph) && wait(&bar.p_full[0], ph);
+        const int next = j + 1;
+        const bool more = next < ntiles;
+        ok = wait(&bar.v_full[j & 1], (j >> 1) & 1) && mma_o(0, j);
         if (!ok) break;
-        dev::tc_fence_after();
-        mma_o(0, j);
         if (!two) dev::umma_commit(&bar.v_empty[j & 1]);
         if (more) {
-          if (!(ok = wait(&bar.k_full[next & 1], nph))) break;
+          if (!(ok = wait(&bar.k_full[next & 1], (next >> 1) & 1))) break;
           dev::tc_fence_after();
           mma_s(0, next);
           dev::umma_commit(&bar.s_full[0]);
           if (!two) dev::umma_commit(&bar.k_empty[next & 1]);
         }
         if (two) {
-          if (!(ok = wait(&bar.p_full[1], ph))) break;
-          dev::tc_fence_after();
-          mma_o(1, j);
+          if (!(ok = mma_o(1, j))) break;
           dev::umma_commit(&bar.v_empty[j & 1]);
           if (more) {
             mma_s(1, next);
@@ -275,143 +400,169 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- converters
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    constexpr int N = DIM / 16;  // 16-code loads per thread, tile and operand
-    const int cw = warp - 8, ct = threadIdx.x - 256;
-    const int lg = a.kv.page_log2;
-    // Lanes take 4 chunks x 8 rows at a time: 64-byte segments from memory and, as neighbouring
-    // rows swizzle to the other parity of 16-byte units, shared-memory stores without conflicts.
-    // Load i: rows cw * 32 + (i / (DIM / 64)) * 8 + lane / 4, chunk (i % (DIM / 64)) * 4 + lane % 4.
-    // Page numbers are fetched two tiles ahead of their use and looked at only then: a check right
-    // after the load would wait for memory twice per tile.
-    int next_pid[2], next_sc = -1;
-    float2 sc = {0.f, 0.f};
-    int sc_ok = 0;
-    // page of the 16 keys from `key` on; -1 where no row of the block sees them
-    auto fetch_pid = [&](int key) -> int {
-      return key < kr.hi && key + 15 >= kr.lo ? __ldg(a.b.table + (size_t)seq * a.b.cols + (key >> lg)) : -1;
-    };
-    // a page number that is out of range is reported, and its keys are not seen
-    auto good = [&](int pid, int key) -> int {
-      if ((unsigned)pid < (unsigned)a.kv.pages) return pid;
-      if (key < kr.hi && key + 15 >= kr.lo) atomicOr(err, ACF_DEV_ERR_BADARG);
-      return -1;
-    };
-    auto fetch = [&](int j) {
-      const int key = (tile0 + j) * kKeys;
-      next_pid[0] = fetch_pid(key + cw * 32);
-      next_pid[1] = fetch_pid(key + cw * 32 + 16);
-      if (ct < kUnits) next_sc = fetch_pid(key + ct * 16);
-    };
-    int pid[2];
-    auto take = [&](int j) {  // the fetched numbers become tile j's; its scales are requested
-      const int key = (tile0 + j) * kKeys;
-      pid[0] = good(next_pid[0], key + cw * 32);
-      pid[1] = good(next_pid[1], key + cw * 32 + 16);
-      if (ct < kUnits) {
-        const int pg = good(next_sc, key + ct * 16);
-        sc_ok = pg >= 0;
-        if (sc_ok) {
-          const size_t at = (size_t)pg * a.kv.heads + head;
-          sc = make_float2(a.kv.ks[at], a.kv.vs[at]);
+    if constexpr (!PRE) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+      constexpr int N = DIM / 16;  // 16-code loads per thread, tile and operand
+      const int cw = warp - 8, ct = threadIdx.x - 256;
+      const int lg = a.kv.page_log2;
+      // Lanes take 4 chunks x 8 rows at a time: 64-byte segments from memory and, as neighbouring
+      // rows swizzle to the other parity of 16-byte units, shared-memory stores without conflicts.
+      // Load i: rows cw * 32 + (i / (DIM / 64)) * 8 + lane / 4, chunk (i % (DIM / 64)) * 4 + lane % 4.
+      // Page numbers are fetched two tiles ahead of their use and looked at only then: a check right
+      // after the load would wait for memory twice per tile.
+      int next_pid[2], next_sc = -1;
+      float2 sc = {0.f, 0.f};
+      int sc_ok = 0;
+      // page of the 16 keys from `key` on; -1 where no row of the block sees them
+      auto fetch_pid = [&](int key) -> int {
+        return key < kr.hi && key + 15 >= kr.lo ? __ldg(a.b.table + (size_t)seq * a.b.cols + (key >> lg)) : -1;
+      };
+      // a page number that is out of range is reported, and its keys are not seen
+      auto good = [&](int pid, int key) -> int {
+        if ((unsigned)pid < (unsigned)a.kv.pages) return pid;
+        if (key < kr.hi && key + 15 >= kr.lo) atomicOr(err, ACF_DEV_ERR_BADARG);
+        return -1;
+      };
+      auto fetch = [&](int j) {
+        const int key = (tile0 + j) * kKeys;
+        next_pid[0] = fetch_pid(key + cw * 32);
+        next_pid[1] = fetch_pid(key + cw * 32 + 16);
+        if (ct < kUnits) next_sc = fetch_pid(key + ct * 16);
+      };
+      int pid[2];
+      auto take = [&](int j) {  // the fetched numbers become tile j's; its scales are requested
+        const int key = (tile0 + j) * kKeys;
+        pid[0] = good(next_pid[0], key + cw * 32);
+        pid[1] = good(next_pid[1], key + cw * 32 + 16);
+        if (ct < kUnits) {
+          const int pg = good(next_sc, key + ct * 16);
+          sc_ok = pg >= 0;
+          if (sc_ok) {
+            const size_t at = (size_t)pg * a.kv.heads + head;
+            sc = make_float2(a.kv.ks[at], a.kv.vs[at]);
+          }
         }
-      }
-    };
-    const int key_in_unit = lane >> 2;
-    auto load_tile = [&](const int8_t* codes, uint4 (&r)[N]) {
+      };
+      const int key_in_unit = lane >> 2;
+      auto load_tile = [&](const int8_t* codes, uint4 (&r)[N]) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int slot = (cw * 32 + u * 16 + key_in_unit) & (a.kv.page - 1);  // tiles start at multiples of every page size
-        const int8_t* src = codes + (((size_t)max(pid[u], 0) * a.kv.heads + head) * a.kv.page + slot) * DIM + (lane & 3) * 16;
+        for (int u = 0; u < 2; ++u) {
+          const int slot = (cw * 32 + u * 16 + key_in_unit) & (a.kv.page - 1);  // tiles start at multiples of every page size
+          const int8_t* src = codes + (((size_t)max(pid[u], 0) * a.kv.heads + head) * a.kv.page + slot) * DIM + (lane & 3) * 16;
 #pragma unroll
-        for (int i = u * N / 2; i < (u + 1) * N / 2; ++i) {
-          r[i] = make_uint4(0, 0, 0, 0);
-          if (pid[u] >= 0)
-            r[i] = __ldg(reinterpret_cast<const uint4*>(src + ((i / L::kChunks) & 1) * 8 * DIM + (i % L::kChunks) * 64));
+          for (int i = u * N / 2; i < (u + 1) * N / 2; ++i) {
+            r[i] = make_uint4(0, 0, 0, 0);
+            if (pid[u] >= 0)
+              r[i] = __ldg(reinterpret_cast<const uint4*>(src + ((i / L::kChunks) & 1) * 8 * DIM + (i % L::kChunks) * 64));
+          }
         }
-      }
-    };
-    // this thread's two 16-byte units of row cw * 32 + lane / 4; its other rows are 8 apart
-    const int unit0 = (cw * 32 + key_in_unit) * 128 + (((2 * (lane & 3)) ^ key_in_unit) << 4);
-    const int unit1 = (cw * 32 + key_in_unit) * 128 + (((2 * (lane & 3) + 1) ^ key_in_unit) << 4);
-    auto put_tile = [&](uint8_t* tile, const uint4 (&r)[N]) {
+      };
+      // this thread's two 16-byte units of row cw * 32 + lane / 4; its other rows are 8 apart
+      const int unit0 = (cw * 32 + key_in_unit) * 128 + (((2 * (lane & 3)) ^ key_in_unit) << 4);
+      const int unit1 = (cw * 32 + key_in_unit) * 128 + (((2 * (lane & 3) + 1) ^ key_in_unit) << 4);
+      auto put_tile = [&](uint8_t* tile, const uint4 (&r)[N]) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int off = (i / L::kChunks) * 8 * 128 + (i % L::kChunks) * (kKeys * 128);
-        put8(tile + unit0 + off, r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u);
-        put8(tile + unit1 + off, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u);
-      }
-    };
-    uint4 kreg[N], vreg[N];
-    if (ntiles > 0) {
-      fetch(0);
-      take(0);
-      if (ntiles > 1) fetch(1);
-      load_tile(a.kv.k, kreg);
-      load_tile(a.kv.v, vreg);
-    }
-    for (int j = 0; j < ntiles; ++j) {
-      const int st = j & 1;
-      const uint32_t eph = ((j >> 1) & 1) ^ 1;
-      const bool more = j + 1 < ntiles;
-      if (!wait(&bar.k_empty[st], eph)) break;
-      put_tile(smem + L::kK + st * L::kTile, kreg);
-      if (ct < kUnits) {
-        // a missing page's keys are masked (past the length) or not seen (out of range)
-        const float vs = fmaxf(sc.y, 0x1p-100f);
-        scales[(j % kScaleRing) * kUnits + ct] =
-            sc_ok ? make_float4(fabsf(a.scale) * sc.x * 1.4426950408889634f, log2f(vs), 1.0f / vs, 0.0f)
-                  : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
-      }
-      dev::fence_proxy_async_smem();
-      arrive(&bar.k_full[st]);
-      if (more) {
-        take(j + 1);
-        if (j + 2 < ntiles) fetch(j + 2);
+        for (int i = 0; i < N; ++i) {
+          const int off = (i / L::kChunks) * 8 * 128 + (i % L::kChunks) * (kKeys * 128);
+          put8(tile + unit0 + off, r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u);
+          put8(tile + unit1 + off, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u);
+        }
+      };
+      uint4 kreg[N], vreg[N];
+      if (ntiles > 0) {
+        fetch(0);
+        take(0);
+        if (ntiles > 1) fetch(1);
         load_tile(a.kv.k, kreg);
+        load_tile(a.kv.v, vreg);
       }
-      if (!wait(&bar.v_empty[st], eph)) break;
-      put_tile(smem + L::kV + st * L::kTile, vreg);
-      dev::fence_proxy_async_smem();
-      arrive(&bar.v_full[st]);
-      if (more) load_tile(a.kv.v, vreg);
+      for (int j = 0; j < ntiles; ++j) {
+        const int st = j & 1;
+        const uint32_t eph = ((j >> 1) & 1) ^ 1;
+        const bool more = j + 1 < ntiles;
+        if (!wait(&bar.k_empty[st], eph)) break;
+        put_tile(smem + L::kK + st * L::kTile, kreg);
+        if (ct < kUnits) {
+          scales[(j % kScaleRing) * kUnits + ct] = scale_entry(sc, sc_ok, a.scale);
+        }
+        dev::fence_proxy_async_smem();
+        arrive(&bar.k_full[st]);
+        if (more) {
+          take(j + 1);
+          if (j + 2 < ntiles) fetch(j + 2);
+          load_tile(a.kv.k, kreg);
+        }
+        if (!wait(&bar.v_empty[st], eph)) break;
+        put_tile(smem + L::kV + st * L::kTile, vreg);
+        dev::fence_proxy_async_smem();
+        arrive(&bar.v_full[st]);
+        if (more) load_tile(a.kv.v, vreg);
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax, one row per thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if constexpr (PRE)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = warp >> 2, row = threadIdx.x & 127;
     const int r = r0 + t * 128 + row;
     const bool in = r < rows;
     const int tok = r / a.group, hq = head * a.group + r - tok * a.group;
     float q_unit = 1.0f;
     {
-      // the row to shared memory as fp16, scaled by a power of two
-      const T* src = static_cast<const T*>(a.q) + (long long)(sv.row0 + tok) * a.q_token + (long long)hq * a.q_head;
-      const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-      float top = 0.0f;
-      if (in) {
+      // Q to shared memory as fp16, each row scaled by a power of two: a warp copies its 32 rows as they
+      // are, all in flight at once, DIM / 8 lanes with 16 bytes of a row each, and converts them in
+      // place, a few rows at a time to cover the latencies of a row's own chain.
+      constexpr int LPR = DIM / 8, RPP = 32 / LPR, N = 32 / RPP;  // lanes per row, rows per pass, passes
+      const int sub = lane / LPR, c = lane % LPR;
+      const T* q = static_cast<const T*>(a.q);
+      const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && a.q_token % 8 == 0 && a.q_head % 8 == 0;
+      const int w0 = (warp & 3) * 32;  // first row of the warp in its tile
+      uint8_t* tile = smem + L::kQ + t * L::kQTile + (c >> 3) * (128 * 128);
+      auto place = [&](int i) -> uint8_t* {
+        const int r = w0 + i * RPP + sub;
+        return tile + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      };
 #pragma unroll 4
-        for (int d = 0; d < DIM; d += 8) {
-          float x[8];
-          load8(src + d, vec, x);
+      for (int i = 0; i < N; ++i) {
+        const int rr = min(r0 + t * 128 + w0 + i * RPP + sub, rows - 1);  // rows past the end repeat the last
+        const int tk = rr / a.group, h = head * a.group + rr - tk * a.group;
+        const T* src = q + (long long)(sv.row0 + tk) * a.q_token + (long long)h * a.q_head + c * 8;
+        if (vec) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dev::smem_u32(place(i))), "l"(src) : "memory");
+        } else {
+          T* o = reinterpret_cast<T*>(place(i));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+          for (int e = 0; e < 8; ++e) o[e] = src[e];
         }
       }
-      int ex = 0;
-      if (top > 0.0f && top <= 3.4028234663852886e38f) frexpf(top, &ex);
-      ex = min(max(ex, -100), 126);
-      const float down = copysignf(exp2f((float)-ex), a.scale);
-      q_unit = exp2f((float)ex);
-      uint8_t* tile = smem + L::kQ + t * L::kQTile + row * 128;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      // each lane converts what it copied itself
 #pragma unroll 4
-      for (int d = 0; d < DIM; d += 8) {
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (in) load8(src + d, vec, x);
+      for (int i = 0; i < N; ++i) {
+        uint4* at = reinterpret_cast<uint4*>(place(i));
+        union {
+          uint4 u;
+          T e[8];
+        } x;
+        x.u = *at;
+        float y[8], top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = to_f(x.e[e]), top = fmaxf(top, fabsf(y[e]));
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const Pow2 f = row_pow2(top);
+        const float down = copysignf(f.down, a.scale);
+#pragma unroll
+        for (int k = 0; k < RPP; ++k) {
+          const float up = __shfl_sync(0xffffffffu, f.up, k * LPR);
+          if (lane == i * RPP + k) q_unit = up;
+        }
         uint4 o;
-        o.x = pack_f16(x[0] * down, x[1] * down), o.y = pack_f16(x[2] * down, x[3] * down);
-        o.z = pack_f16(x[4] * down, x[5] * down), o.w = pack_f16(x[6] * down, x[7] * down);
-        *reinterpret_cast<uint4*>(tile + (d >> 6) * (128 * 128) + ((((d >> 3) & 7) ^ (row & 7)) << 4)) = o;
+        o.x = pack_f16(y[0] * down, y[1] * down), o.y = pack_f16(y[2] * down, y[3] * down);
+        o.z = pack_f16(y[4] * down, y[5] * down), o.w = pack_f16(y[6] * down, y[7] * down);
+        *at = o;
       }
       dev::fence_proxy_async_smem();
       arrive(&bar.q_full);
@@ -460,6 +611,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
         l *= b;
       }
       const float m0 = m == -INFINITY ? 0.0f : m;
+      if (move && j > 0) {  // S of tile j was issued after O's product of tile j - 1, which is done
+#pragma unroll 1
+        for (int i = 0; i < DIM / 16; ++i) {
+          float o[16];
+          tmem_ld16p(tO0 + t * DIM + lanes + i * 16, o);
+          dev::tmem_ld_wait();
+          uint32_t x[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * b);
+          tmem_st16(tO0 + t * DIM + lanes + i * 16, x);
+        }
+      }
 #pragma unroll
       for (int h = 0; h < 4; ++h) {  // 32 keys: 16 registers of weights
         uint32_t w[16];
@@ -473,34 +636,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             float2 e = fma2(make_float2(s[16 * u + i], s[16 * u + i + 1]), fx2, off2);
-            e.x = ex2(e.x), e.y = ex2(e.y);
+            if ((i / 2) % 4 >= kFmaOf4) {
+              e.x = ex2(e.x), e.y = ex2(e.y);
+            } else {
+              e = ex2_fma2(e);
+            }
             sum = add2(sum, e);
             w[8 * v + i / 2] = pack_f16(e.x, e.y);
           }
           l = fmaf(sum.x + sum.y, f.z, l);
         }
         tmem_st16(tS0 + t * 128 + lanes + 16 * h, w);
-      }
-      if (move && j > 0) {  // S of tile j was issued after O's product of tile j - 1, which is done
-#pragma unroll 1
-        for (int i = 0; i < DIM / 32; ++i) {
-          float o[32];
-          tmem_ld32p(tO0 + t * DIM + lanes + i * 32, o);
-          dev::tmem_ld_wait();
-          uint32_t x[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(o[e] * b);
-          tmem_st32(tO0 + t * DIM + lanes + i * 32, x);
+        if (h & 1) {
+          tmem_st_wait();
+          dev::tc_fence_before();
+          arrive(&bar.p_full[t][h >> 1]);
         }
       }
-      tmem_st_wait();
-      dev::tc_fence_before();
-      arrive(&bar.p_full[t]);
     }
     if (ok && ntiles > 0) ok = wait(&bar.o_full, 0);
     dev::tc_fence_after();
     if (active) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      // no key seen: m is -inf and l holds at most the least powers of two (a NaN has m = -inf too)
+      const bool none = ntiles == 0 || (m == -INFINITY && l == l);
+      const float inv = none ? 0.0f : 1.0f / l;
       const bool whole = nsplit == 1;
       T* dst = static_cast<T*>(a.out) + (long long)(sv.row0 + tok) * a.o_token + (long long)hq * a.o_head;
       const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
@@ -521,27 +680,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const TcArgs p, unsig
           for (int e = 0; e < 32; e += 8) {
             float x[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = l == 0.0f ? 0.0f : o[e + k] * inv;
+            for (int k = 0; k < 8; ++k) x[k] = none ? 0.0f : o[e + k] * inv;
             store8(dst + i * 32 + e, vec, x);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(p.part_o + at * DIM + i * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            *reinterpret_cast<float4*>(p.part_o + at * DIM + i * 32 + e) = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       }
       if (in && ok) {
         if (!whole)
-          p.part_ml[at] = make_float2(m, l);
+          p.part_ml[at] = make_float2(m, none ? 0.0f : l);
         else if (a.lse)
           a.lse[(long long)(sv.row0 + tok) * a.q_heads + hq] =
-              l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+              none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
       }
     }
   }
   dev::tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == Roles<PRE>::kMmaWarp) {
     dev::tc_fence_after();
     dev::tmem_dealloc(tmem, 512);
   }
@@ -579,34 +738,53 @@ __global__ void __launch_bounds__(128) k_attn_join(const TcArgs p, unsigned* err
     a.lse[(long long)(sv.row0 + tok) * a.q_heads + hq] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
-template <typename T, int DIM>
-bool tc_launch(Call& c, const AttnArgs& a) {
+template <typename T, int DIM, bool PRE>
+bool tc_launch(Call& c, TcArgs p, dim3 grid) {
   using L = TcSmem<DIM>;
   static bool attr_done[64] = {false};
   const int dv = current_device() & 63;
   if (!attr_done[dv]) {
-    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_tc<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes)))
+    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_tc<T, DIM, PRE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes)))
       return false;
     attr_done[dv] = true;
   }
+  k_attn_tc<T, DIM, PRE><<<grid, Roles<PRE>::kThreads, L::kBytes, c.stream()>>>(p, c.err());
+  return c.launched("k_attn_tc");
+}
+
+template <typename T, int DIM>
+bool tc_run(Call& c, const AttnArgs& a) {
   TcArgs p = {};
   p.a = a;
   const long long max_new = std::min(a.b.max_new, a.b.tokens);
   p.row_tiles = (int)((max_new * a.group + kRows - 1) / kRows);
   // few blocks: the keys are split so that every SM gets one, in parts of at least 4 key tiles
   const long long work = (long long)p.row_tiles * a.kv.heads * a.b.seqs;
-  const int tiles = (a.b.max_len + kKeys - 1) / kKeys + 1;  // a window can start inside a tile
+  const int tiles = (a.b.max_len + kKeys - 1) / kKeys;
   const long long want = std::max<long long>(1, c.sm_count() / std::max<long long>(1, work));
-  p.chunk = (int)std::max<long long>(4, (tiles + want - 1) / want);
-  p.splits = (tiles + p.chunk - 1) / p.chunk;
+  p.chunk = (int)std::max<long long>(4, (tiles + 1 + want - 1) / want);
+  p.splits = (tiles + 1 + p.chunk - 1) / p.chunk;  // a window can start inside a tile
   if (p.splits > 1) {
     const size_t n = (size_t)a.b.tokens * a.q_heads * p.splits;
     p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
     p.part_ml = (float2*)c.scratch(n * sizeof(float2));
     if (!c.ok()) return false;
   }
-  k_attn_tc<T, DIM><<<dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), kTcThreads, L::kBytes, c.stream()>>>(p, c.err());
-  if (!c.launched("k_attn_tc")) return false;
+  // tile images before the kernel: where the conversion would be repeated, and they fit
+  const size_t images = (size_t)a.b.seqs * a.kv.heads * tiles;
+  const bool pre = p.row_tiles >= kPreRowTiles && images * (2 * kKeys * DIM * 2) <= kPreBytes;
+  const dim3 grid(p.row_tiles * a.kv.heads, a.b.seqs, p.splits);
+  if (pre) {
+    p.tiles = tiles;
+    p.k_img = (uint8_t*)c.scratch(images * kKeys * DIM * 2);
+    p.v_img = (uint8_t*)c.scratch(images * kKeys * DIM * 2);
+    p.scale_img = (float4*)c.scratch(images * kUnits * sizeof(float4));
+    if (!c.ok()) return false;
+    k_kv8_tiles<DIM><<<dim3(tiles, a.kv.heads, a.b.seqs), 256, 0, c.stream()>>>(p, c.err());
+    if (!c.launched("k_kv8_tiles") || !tc_launch<T, DIM, true>(c, p, grid)) return false;
+  } else if (!tc_launch<T, DIM, false>(c, p, grid)) {
+    return false;
+  }
   if (p.splits > 1) {
     const long long items = (max_new * a.q_heads + 3) / 4;
     k_attn_join<T, DIM><<<dim3((unsigned)items, a.b.seqs), 128, 0, c.stream()>>>(p, c.err());
@@ -618,8 +796,8 @@ bool tc_launch(Call& c, const AttnArgs& a) {
 }  // namespace
 
 bool attn_tc_dev(Call& c, const AttnArgs& a) {
-  if (a.dtype == ACFUN_F16) return a.kv.dim == 64 ? tc_launch<__half, 64>(c, a) : tc_launch<__half, 128>(c, a);
-  return a.kv.dim == 64 ? tc_launch<__nv_bfloat16, 64>(c, a) : tc_launch<__nv_bfloat16, 128>(c, a);
+  if (a.dtype == ACFUN_F16) return a.kv.dim == 64 ? tc_run<__half, 64>(c, a) : tc_run<__half, 128>(c, a);
+  return a.kv.dim == 64 ? tc_run<__nv_bfloat16, 64>(c, a) : tc_run<__nv_bfloat16, 128>(c, a);
 }
 
 bool attn_tc_takes(const AttnArgs& a) {

@@ -27,6 +27,17 @@ __device__ __forceinline__ KeyRange key_range(const AttnArgs& a, const SeqView& 
   return k;
 }
 
+// The power of two that brings a row whose largest element is `top` below 1, and its inverse.  A row
+// with an infinity or NaN is left as it is.
+struct Pow2 {
+  float down, up;
+};
+__device__ __forceinline__ Pow2 row_pow2(float top) {
+  const int biased = (int)(__float_as_uint(top) >> 23);  // 0: zero or subnormal, 255: not finite
+  const int ex = biased == 255 ? 0 : min(max(biased - 126, -100), 126);
+  return {__uint_as_float((uint32_t)(127 - ex) << 23), __uint_as_float((uint32_t)(127 + ex) << 23)};
+}
+
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
