@@ -14,11 +14,13 @@
 //                   a row per thread)
 // The codes become fp16 in the 128-byte swizzled layout of the MMA operands in one of two places:
 //   in the kernel   warps 8-11 convert the block's keys one tile ahead (two stages each for K and V),
-//                   warp 12 issues the MMAs; the cache is read once per 256 rows, at one byte a code
-//   before it       k_kv8_tiles writes each key tile's image to scratch once, and warp 9 only copies
-//                   images (cp.async.bulk), warp 8 issues the MMAs.  Conversion costs the softmax's
+//                   warps 12 and 13 issue the MMAs; the cache is read once per 256 rows, at one byte a code
+//   before it       k_kv8_tiles writes each key tile's image to scratch once, and warp 10 only copies
+//                   images (cp.async.bulk), warps 8 and 9 issue the MMAs.  Conversion costs the softmax's
 //                   issue slots and registers, and with many row tiles it is repeated for each.
-// TMEM: S of A and B (128 columns each; the fp16 weights overlay their first half), O of A and B.
+// TMEM: two buffers of S of A and of B (64 keys, 64 columns each; the fp16 weights overlay their
+// first half), O of A and B.  With one buffer of 128 keys a softmax waited a third of its time for
+// the products between its weights and its next scores.
 // Every wait is bounded (ptx.cuh); on expiry the error word is set and all roles leave.
 #include <math.h>
 
@@ -35,14 +37,15 @@ template <bool PRE>
 struct Roles;
 template <>
 struct Roles<false> {
-  static constexpr int kThreads = 512, kMmaWarp = 12;  // 2 x 168 + 112 + 64 = 4 x 128
+  static constexpr int kThreads = 512, kMmaWarp = 12, kMmaWarpB = 13;  // 2 x 144 + 128 + 96 = 4 x 128
 };
 template <>
 struct Roles<true> {
-  static constexpr int kThreads = 384, kMmaWarp = 8, kCopyWarp = 9;  // 2 x 216 + 72 = 3 x 168
+  static constexpr int kThreads = 384, kMmaWarp = 8, kMmaWarpB = 9, kCopyWarp = 10;  // 2 x 192 + 120 = 3 x 168
 };
 constexpr int kRows = 256;     // packed rows of a block
-constexpr int kKeys = 128;     // keys per step
+constexpr int kKeys = 128;     // keys per stage of K and V
+constexpr int kStep = 64;      // keys of one S product and its softmax
 constexpr int kUnits = kKeys / 16;
 constexpr int kFmaOf4 = 1;      // pairs of four whose 2^x the FMA units compute instead of the special function unit
 constexpr float kLeast = 1e-37f;  // a factor never underflows to 0: a masked score stays -inf under it
@@ -77,7 +80,7 @@ struct TcSmem {
 
 struct TcBars {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2][2], o_full, drain;
+  uint64_t s_full[2][2], p_full[2][2], o_step[2], o_full, drain[2];  // [tile][buffer of S]
   uint32_t tmem;
   volatile int abort;
 };
@@ -251,21 +254,26 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
   const int nsplit = max(1, (kr.n + p.chunk - 1) / p.chunk);
   if (part >= nsplit) return;
   const int tile0 = kr.first + part * p.chunk, ntiles = min(kr.n - part * p.chunk, p.chunk);
+  // steps of 64 keys; the last key tile may need its first half only
+  const int steps = ntiles > 0 ? min(2 * ntiles, (kr.hi - tile0 * kKeys + kStep - 1) / kStep) : 0;
   const bool two = nr > 128;
 
   if (threadIdx.x == 0) {
     dev::mbar_init(&bar.q_full, 8);
     for (int i = 0; i < 2; ++i) {
       dev::mbar_init(&bar.k_full[i], PRE ? 1 : 4);
-      dev::mbar_init(&bar.k_empty[i], 1);
+      dev::mbar_init(&bar.k_empty[i], two ? 2 : 1);
       dev::mbar_init(&bar.v_full[i], PRE ? 1 : 4);
-      dev::mbar_init(&bar.v_empty[i], 1);
-      dev::mbar_init(&bar.s_full[i], 1);
+      dev::mbar_init(&bar.v_empty[i], two ? 2 : 1);
+      dev::mbar_init(&bar.s_full[i][0], 1);
+      dev::mbar_init(&bar.s_full[i][1], 1);
+      dev::mbar_init(&bar.o_step[i], 1);
       dev::mbar_init(&bar.p_full[i][0], 4);
       dev::mbar_init(&bar.p_full[i][1], 4);
     }
-    dev::mbar_init(&bar.o_full, 1);
-    dev::mbar_init(&bar.drain, 1);
+    dev::mbar_init(&bar.o_full, two ? 2 : 1);
+    dev::mbar_init(&bar.drain[0], 1);
+    dev::mbar_init(&bar.drain[1], 1);
     bar.abort = 0;
     dev::fence_mbar_init();
   }
@@ -294,9 +302,9 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
   if (warp >= (PRE ? 8 : 12)) {
     // ---------------------------------------------------------------- MMA issuer, image copies
     if constexpr (PRE)
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     else
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if constexpr (PRE) {
       if (warp == Roles<PRE>::kCopyWarp && dev::elect_one()) {
         const size_t at = ((size_t)seq * a.kv.heads + head) * p.tiles + tile0;
@@ -307,6 +315,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
           dev::mbar_arrive_expect_tx(&bar.k_full[st], L::kTile + kUnits * 16);
           dev::bulk_load(smem + L::kK + st * L::kTile, p.k_img + (at + j) * L::kTile, L::kTile, &bar.k_full[st]);
           dev::bulk_load(scales + (j % kScaleRing) * kUnits, p.scale_img + (at + j) * kUnits, kUnits * 16, &bar.k_full[st]);
+          // the first product needs Q and the first K tile: what follows waits until Q is there
+          if (j == 0 && !wait(&bar.q_full, 0)) break;
           if (!wait(&bar.v_empty[st], eph)) break;
           dev::mbar_arrive_expect_tx(&bar.v_full[st], L::kTile);
           dev::bulk_load(smem + L::kV + st * L::kTile, p.v_img + (at + j) * L::kTile, L::kTile, &bar.v_full[st]);
@@ -322,12 +332,16 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
     // The issuing thread is one that elect.sync names: with a thread picked by its lane number the
     // compiler has to move every operand to uniform registers by itself, and next to busy softmax
     // warps an instruction then took 116 cycles to issue instead of the 64 that it runs.
-    if (warp == Roles<PRE>::kMmaWarp && ntiles > 0 && dev::elect_one()) {
-      constexpr uint32_t idS = dev::umma_idesc(1, 0, 0, 0, 0, 128, kKeys), idO = dev::umma_idesc(1, 0, 0, 0, 1, 128, DIM);
+    // Each tile has an issuer of its own: a wait costs one 100 cycles and more even when it is over,
+    // and the other's products run meanwhile.
+    const int t = warp == Roles<PRE>::kMmaWarpB;
+    if ((warp == Roles<PRE>::kMmaWarp || (t && two)) && steps > 0 && dev::elect_one()) {
+      constexpr uint32_t idS = dev::umma_idesc(1, 0, 0, 0, 0, 128, kStep), idO = dev::umma_idesc(1, 0, 0, 0, 1, 128, DIM);
       const uint32_t base = dev::smem_u32(smem);
-      const uint64_t dQ = dev::umma_sdesc(base + L::kQ, 16, 1024, dev::UMMA_SW128);
+      const uint64_t dQ = dev::umma_sdesc(base + L::kQ + t * L::kQTile, 16, 1024, dev::UMMA_SW128);
       const uint64_t dK = dev::umma_sdesc(base + L::kK, 16, 1024, dev::UMMA_SW128);
       const uint64_t dV = dev::umma_sdesc(base + L::kV, kKeys * 128, 1024, dev::UMMA_SW128);
+      const uint32_t tS = tS0 + t * 128, tO = tO0 + t * DIM;
       // Descriptors are formed anew for each group of products: left to itself the compiler keeps all
       // of them across the loop, which in this role's registers means local memory, and a load from it
       // per instruction made the products of S four times as long as the tensor cores take.
@@ -336,73 +350,53 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
         asm volatile("mov.b64 %0, %1;" : "=l"(r) : "l"(d));
         return r;
       };
-      auto mma_s = [&](int t, int j) {  // S of tile t against key tile j
-        const uint64_t q = fresh(dQ + ((t * L::kQTile) >> 4)), k = fresh(dK + (((j & 1) * L::kTile) >> 4));
+      // S for the 64 keys of step i, into the buffer of the step's parity
+      auto mma_s = [&](int i) {
+        const uint64_t q = fresh(dQ);
+        const uint64_t k = fresh(dK + ((((i >> 1) & 1) * L::kTile + (i & 1) * kStep * 128) >> 4));
 #pragma unroll
         for (int ks = 0; ks < DIM / 16; ++ks) {
           const uint32_t off = ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32) >> 4;
-          dev::umma<dev::MmaKind::F16>(tS0 + t * 128, q + off, k + off, idS, ks != 0);
+          dev::umma<dev::MmaKind::F16>(tS + (i & 1) * kStep, q + off, k + off, idS, ks != 0);
         }
-      };
-      auto mma_o = [&](int t, int j) -> bool {  // the weights of a tile come in two halves of 64 keys
-        const uint64_t v = fresh(dV + (((j & 1) * L::kTile) >> 4));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!wait(&bar.p_full[t][h], j & 1)) return false;
-          dev::tc_fence_after();
-#pragma unroll
-          for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
-            umma_ts_f16(tO0 + t * DIM, tS0 + t * 128 + ks * 8, v + ((ks * 2048) >> 4), idO, (j | ks) != 0);
-        }
-        return true;
+        dev::umma_commit(&bar.s_full[t][i & 1]);
       };
       bool ok = wait(&bar.q_full, 0) && wait(&bar.k_full[0], 0);
       dev::tc_fence_after();
-      if (ok) {
-        mma_s(0, 0);
-        dev::umma_commit(&bar.s_full[0]);
-        if (two) {
-          mma_s(1, 0);
-          dev::umma_commit(&bar.s_full[1]);
-        }
-        dev::umma_commit(&bar.k_empty[0]);
+      for (int i = 0; i < min(steps, 2) && ok; ++i) {
+        mma_s(i);
+        if (i == 1) dev::umma_commit(&bar.k_empty[0]);
       }
-      for (int j = 0; j < ntiles && ok; ++j) {
-        const int next = j + 1;
-        const bool more = next < ntiles;
-        ok = wait(&bar.v_full[j & 1], (j >> 1) & 1) && mma_o(0, j);
-        if (!ok) break;
-        if (!two) dev::umma_commit(&bar.v_empty[j & 1]);
-        if (more) {
-          if (!(ok = wait(&bar.k_full[next & 1], (next >> 1) & 1))) break;
-          dev::tc_fence_after();
-          mma_s(0, next);
-          dev::umma_commit(&bar.s_full[0]);
-          if (!two) dev::umma_commit(&bar.k_empty[next & 1]);
-        }
-        if (two) {
-          if (!(ok = mma_o(1, j))) break;
-          dev::umma_commit(&bar.v_empty[j & 1]);
-          if (more) {
-            mma_s(1, next);
-            dev::umma_commit(&bar.s_full[1]);
-            dev::umma_commit(&bar.k_empty[next & 1]);
-          }
+      // S runs two steps ahead of O, so a softmax finds its next scores when it is done with the last
+      for (int i = 0; i < steps; ++i) {
+        const int n = i + 2, j = i >> 1, jn = n >> 1;
+        if (ok && !(i & 1)) ok = wait(&bar.v_full[j & 1], (j >> 1) & 1);
+        if (ok && n < steps && !(n & 1)) ok = wait(&bar.k_full[jn & 1], (jn >> 1) & 1);
+        if (!(ok = ok && wait(&bar.p_full[t][i & 1], j & 1))) break;
+        dev::tc_fence_after();
+        const uint64_t v = fresh(dV + (((j & 1) * L::kTile + (i & 1) * kStep * 128) >> 4));
+#pragma unroll
+        for (int ks = 0; ks < kStep / 16; ++ks)
+          umma_ts_f16(tO, tS + (i & 1) * kStep + ks * 8, v + ((ks * 2048) >> 4), idO, (i | ks) != 0);
+        dev::umma_commit(&bar.o_step[t]);
+        if (i & 1) dev::umma_commit(&bar.v_empty[j & 1]);
+        if (n < steps) {
+          mma_s(n);
+          if (n & 1) dev::umma_commit(&bar.k_empty[jn & 1]);
         }
       }
       if (ok) {
         dev::umma_commit(&bar.o_full);
       } else {
         bar.abort = 1;
-        dev::umma_commit(&bar.drain);
-        dev::mbar_wait(&bar.drain, 0, nullptr, 200000000ull);
+        dev::umma_commit(&bar.drain[t]);
+        dev::mbar_wait(&bar.drain[t], 0, nullptr, 200000000ull);
       }
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- converters
     if constexpr (!PRE) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-      constexpr int N = DIM / 16;  // 16-code loads per thread, tile and operand
+        constexpr int N = DIM / 16;  // 16-code loads per thread, tile and operand
       const int cw = warp - 8, ct = threadIdx.x - 256;
       const int lg = a.kv.page_log2;
       // Lanes take 4 chunks x 8 rows at a time: 64-byte segments from memory and, as neighbouring
@@ -502,9 +496,9 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
   } else {
     // ---------------------------------------------------------------- softmax, one row per thread
     if constexpr (PRE)
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int t = warp >> 2, row = threadIdx.x & 127;
     const int r = r0 + t * 128 + row;
     const bool in = r < rows;
@@ -574,57 +568,57 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     const bool active = t == 0 || two;
-    for (int j = 0; j < ntiles && active; ++j) {
-      if (!(ok = wait(&bar.s_full[t], j & 1))) break;
+    for (int i = 0; i < steps && active; ++i) {
+      const uint32_t tS = tS0 + t * 128 + (i & 1) * kStep + lanes;
+      if (!(ok = wait(&bar.s_full[t][i & 1], (i >> 1) & 1))) break;
       dev::tc_fence_after();
-      float s[kKeys];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32p(tS0 + t * 128 + lanes + i * 32, s + 32 * i);
+      float s[kStep];
+      tmem_ld32p(tS, s);
+      tmem_ld32p(tS + 32, s + 32);
       dev::tmem_ld_wait();
-      const float4* sc = scales + (j % kScaleRing) * kUnits;
-      const int k0 = (tile0 + j) * kKeys;
+      const float4* sc = scales + ((i >> 1) % kScaleRing) * kUnits + (i & 1) * (kUnits / 2);
+      const int k0 = tile0 * kKeys + i * kStep;
       const int lo = see_lo - k0, hi = see_hi - k0;
-      if (__any_sync(0xffffffffu, lo > 0 || hi < kKeys)) {
-        // opaque bounds: the comparisons stay inside this branch instead of running for every tile
+      if (__any_sync(0xffffffffu, lo > 0 || hi < kStep)) {
+        // opaque bounds: the comparisons stay inside this branch instead of running for every step
         int from = lo, to = hi;
         asm volatile("" : "+r"(from), "+r"(to));
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i)
-          if (i < from || i >= to) s[i] = -INFINITY;
+        for (int e = 0; e < kStep; ++e)
+          if (e < from || e >= to) s[e] = -INFINITY;
       }
       float top = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
+      for (int u = 0; u < kStep / 16; ++u) {
         const float* v = s + 16 * u;
         const float x0 = max3(max3(v[0], v[1], v[2]), v[3], v[4]), x1 = max3(max3(v[5], v[6], v[7]), v[8], v[9]);
         const float x2 = max3(max3(v[10], v[11], v[12]), v[13], v[14]);
-        const float x = max3(fmaxf(x0, v[15]), x1, x2);
         const float4 f = sc[u];
-        top = fmaxf(top, fmaf(x, fmaxf(f.x * q_unit, kLeast), f.y));
+        top = fmaxf(top, fmaf(max3(fmaxf(x0, v[15]), x1, x2), fmaxf(f.x * q_unit, kLeast), f.y));
       }
-      float b = 1.0f;
-      const bool move = __any_sync(0xffffffffu, top > m + kMost);
-      if (move) {
+      if (__any_sync(0xffffffffu, top > m + kMost)) {
         const float n = fmaxf(m, top - kTop);
-        b = m == n ? 1.0f : ex2(m - n);
+        const float b = m == n ? 1.0f : ex2(m - n);
         m = n;
         l *= b;
-      }
-      const float m0 = m == -INFINITY ? 0.0f : m;
-      if (move && j > 0) {  // S of tile j was issued after O's product of tile j - 1, which is done
+        if (i > 0) {  // O holds the steps before this one, once the last of them is done
+          if (!(ok = wait(&bar.o_step[t], (i - 1) & 1))) break;
+          dev::tc_fence_after();
 #pragma unroll 1
-        for (int i = 0; i < DIM / 16; ++i) {
-          float o[16];
-          tmem_ld16p(tO0 + t * DIM + lanes + i * 16, o);
-          dev::tmem_ld_wait();
-          uint32_t x[16];
+          for (int c = 0; c < DIM / 16; ++c) {
+            float o[16];
+            tmem_ld16p(tO0 + t * DIM + lanes + c * 16, o);
+            dev::tmem_ld_wait();
+            uint32_t x[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * b);
-          tmem_st16(tO0 + t * DIM + lanes + i * 16, x);
+            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * b);
+            tmem_st16(tO0 + t * DIM + lanes + c * 16, x);
+          }
         }
       }
+      const float m0 = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {  // 32 keys: 16 registers of weights
+      for (int h = 0; h < kStep / 32; ++h) {  // 32 keys: 16 registers of weights
         uint32_t w[16];
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
@@ -634,25 +628,23 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
           const float2 fx2 = make_float2(fx, fx), off2 = make_float2(off, off);
           float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float2 e = fma2(make_float2(s[16 * u + i], s[16 * u + i + 1]), fx2, off2);
-            if ((i / 2) % 4 >= kFmaOf4) {
-              e.x = ex2(e.x), e.y = ex2(e.y);
+          for (int e = 0; e < 16; e += 2) {
+            float2 x = fma2(make_float2(s[16 * u + e], s[16 * u + e + 1]), fx2, off2);
+            if ((e / 2) % 4 >= kFmaOf4) {
+              x.x = ex2(x.x), x.y = ex2(x.y);
             } else {
-              e = ex2_fma2(e);
+              x = ex2_fma2(x);
             }
-            sum = add2(sum, e);
-            w[8 * v + i / 2] = pack_f16(e.x, e.y);
+            sum = add2(sum, x);
+            w[8 * v + e / 2] = pack_f16(x.x, x.y);
           }
           l = fmaf(sum.x + sum.y, f.z, l);
         }
-        tmem_st16(tS0 + t * 128 + lanes + 16 * h, w);
-        if (h & 1) {
-          tmem_st_wait();
-          dev::tc_fence_before();
-          arrive(&bar.p_full[t][h >> 1]);
-        }
+        tmem_st16(tS + 16 * h, w);
       }
+      tmem_st_wait();
+      dev::tc_fence_before();
+      arrive(&bar.p_full[t][i & 1]);
     }
     if (ok && ntiles > 0) ok = wait(&bar.o_full, 0);
     dev::tc_fence_after();
