@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tile.cuh"
 
@@ -184,9 +185,23 @@ __device__ __forceinline__ float4 scale_entry(float2 ks_vs, bool there, float sc
                : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
 }
 
+// Eight codes as T (exact in either type), one 16-byte unit; negated where `flip` is 0x80008000.
+template <typename T>
+__device__ __forceinline__ void put8_as(uint8_t* p, uint32_t w0, uint32_t w1, uint32_t flip) {
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (i < 2 ? w0 : w1) >> (16 * (i & 1));
+    const T lo = from_f<T>((float)(int8_t)w), hi = from_f<T>((float)(int8_t)(w >> 8));
+    o[i] = ((uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16) ^ flip;
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 // Images of the key tiles that some row of a sequence sees: block (tile, head, sequence), 256
-// threads, half of them for K and half for V.  Bound by the write of two bytes per code.
-template <int DIM>
+// threads, half of them for K and half for V.  K takes q's type, so that q is used as it is, and the
+// sign of the scale; V is fp16 as the weights are.  Bound by the write of two bytes per code.
+template <typename T, int DIM>
 __global__ void __launch_bounds__(256) k_kv8_tiles(const TcArgs p, unsigned* err) {
   const AttnArgs& a = p.a;
   const int tile = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
@@ -229,8 +244,14 @@ __global__ void __launch_bounds__(256) k_kv8_tiles(const TcArgs p, unsigned* err
     const int row = r * STEP + r0;
     uint8_t* o = img + (c >> 2) * (kKeys * 128) + row * 128;
     const int x = row & 7, u = 2 * (c & 3);
-    put8(o + ((u ^ x) << 4), w[r].x ^ 0x80808080u, w[r].y ^ 0x80808080u);
-    put8(o + (((u + 1) ^ x) << 4), w[r].z ^ 0x80808080u, w[r].w ^ 0x80808080u);
+    if (v) {
+      put8(o + ((u ^ x) << 4), w[r].x ^ 0x80808080u, w[r].y ^ 0x80808080u);
+      put8(o + (((u + 1) ^ x) << 4), w[r].z ^ 0x80808080u, w[r].w ^ 0x80808080u);
+    } else {
+      const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+      put8_as<T>(o + ((u ^ x) << 4), w[r].x, w[r].y, flip);
+      put8_as<T>(o + (((u + 1) ^ x) << 4), w[r].z, w[r].w, flip);
+    }
   }
 }
 
@@ -336,7 +357,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
     // and the other's products run meanwhile.
     const int t = warp == Roles<PRE>::kMmaWarpB;
     if ((warp == Roles<PRE>::kMmaWarp || (t && two)) && steps > 0 && dev::elect_one()) {
-      constexpr uint32_t idS = dev::umma_idesc(1, 0, 0, 0, 0, 128, kStep), idO = dev::umma_idesc(1, 0, 0, 0, 1, 128, DIM);
+      constexpr uint32_t kQType = PRE && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;  // of Q and K: bf16 or f16
+      constexpr uint32_t idS = dev::umma_idesc(1, kQType, kQType, 0, 0, 128, kStep), idO = dev::umma_idesc(1, 0, 0, 0, 1, 128, DIM);
       const uint32_t base = dev::smem_u32(smem);
       const uint64_t dQ = dev::umma_sdesc(base + L::kQ + t * L::kQTile, 16, 1024, dev::UMMA_SW128);
       const uint64_t dK = dev::umma_sdesc(base + L::kK, 16, 1024, dev::UMMA_SW128);
@@ -505,9 +527,9 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
     const int tok = r / a.group, hq = head * a.group + r - tok * a.group;
     float q_unit = 1.0f;
     {
-      // Q to shared memory as fp16, each row scaled by a power of two: a warp copies its 32 rows as they
-      // are, all in flight at once, DIM / 8 lanes with 16 bytes of a row each, and converts them in
-      // place, a few rows at a time to cover the latencies of a row's own chain.
+      // Q to shared memory: a warp copies its 32 rows as they are, all in flight at once, DIM / 8 lanes
+      // with 16 bytes of a row each.  Where K is fp16 whatever q is, the rows are then converted in
+      // place, each scaled by a power of two.
       constexpr int LPR = DIM / 8, RPP = 32 / LPR, N = 32 / RPP;  // lanes per row, rows per pass, passes
       const int sub = lane / LPR, c = lane % LPR;
       const T* q = static_cast<const T*>(a.q);
@@ -518,21 +540,27 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
         const int r = w0 + i * RPP + sub;
         return tile + r * 128 + (((c & 7) ^ (r & 7)) << 4);
       };
-#pragma unroll 4
+      int rr = r0 + t * 128 + w0 + sub;
+      int h = rr % a.group;
+      const T* src = q + (long long)(sv.row0 + rr / a.group) * a.q_token + (long long)(head * a.group + h) * a.q_head + c * 8;
+#pragma unroll 1
       for (int i = 0; i < N; ++i) {
-        const int rr = min(r0 + t * 128 + w0 + i * RPP + sub, rows - 1);  // rows past the end repeat the last
-        const int tk = rr / a.group, h = head * a.group + rr - tk * a.group;
-        const T* src = q + (long long)(sv.row0 + tk) * a.q_token + (long long)h * a.q_head + c * 8;
-        if (vec) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dev::smem_u32(place(i))), "l"(src) : "memory");
-        } else {
-          T* o = reinterpret_cast<T*>(place(i));
+        if (rr < rows) {
+          if (vec) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dev::smem_u32(place(i))), "l"(src) : "memory");
+          } else {
+            T* o = reinterpret_cast<T*>(place(i));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = src[e];
+            for (int e = 0; e < 8; ++e) o[e] = src[e];
+          }
+        } else {
+          *reinterpret_cast<uint4*>(place(i)) = make_uint4(0, 0, 0, 0);
         }
+        rr += RPP, h += RPP, src += RPP * a.q_head;
+        while (h >= a.group) h -= a.group, src += a.q_token - a.group * a.q_head;
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      // each lane converts what it copied itself
+      if constexpr (!PRE) {  // each lane converts what it copied itself
 #pragma unroll 4
       for (int i = 0; i < N; ++i) {
         uint4* at = reinterpret_cast<uint4*>(place(i));
@@ -557,6 +585,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
         o.x = pack_f16(y[0] * down, y[1] * down), o.y = pack_f16(y[2] * down, y[3] * down);
         o.z = pack_f16(y[4] * down, y[5] * down), o.w = pack_f16(y[6] * down, y[7] * down);
         *at = o;
+      }
       }
       dev::fence_proxy_async_smem();
       arrive(&bar.q_full);
@@ -772,7 +801,7 @@ bool tc_run(Call& c, const AttnArgs& a) {
     p.v_img = (uint8_t*)c.scratch(images * kKeys * DIM * 2);
     p.scale_img = (float4*)c.scratch(images * kUnits * sizeof(float4));
     if (!c.ok()) return false;
-    k_kv8_tiles<DIM><<<dim3(tiles, a.kv.heads, a.b.seqs), 256, 0, c.stream()>>>(p, c.err());
+    k_kv8_tiles<T, DIM><<<dim3(tiles, a.kv.heads, a.b.seqs), 256, 0, c.stream()>>>(p, c.err());
     if (!c.launched("k_kv8_tiles") || !tc_launch<T, DIM, true>(c, p, grid)) return false;
   } else if (!tc_launch<T, DIM, false>(c, p, grid)) {
     return false;
