@@ -92,12 +92,13 @@ struct StreamSmem {
   float2 ml[kWarps][16];
   float row_ml[16][2];
   int last;
+  uint4 q[DIM / 16][32];  // Q fragments, the same for the four warps
   float o[kWarps][16][DIM + 4];
 };
 
 // DIM / 64 runs of 16 bytes per key for K; DIM / 8 bytes per key for V.
 template <typename T, int DIM>
-__global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p, unsigned* err) {
+__global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : 4) k_attn_stream(const StreamArgs p, unsigned* err) {
   constexpr int KR = DIM / 64;          // 16-byte runs of a thread per key (K)
   constexpr int NT = DIM / 8;           // output n-tiles
   constexpr int VW = DIM / 32;          // 32-bit words of a thread per key (V)
@@ -124,77 +125,15 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
   const int lg = a.kv.page_log2;
   const int pg0 = (ub * kUnit) >> lg;
   const int npg = ue > ub ? (((ue * kUnit - 1) >> lg) - pg0 + 1) : 0;
-  for (int i = threadIdx.x; i < npg; i += blockDim.x) {
-    PageEntry e = {-1, 0.0f, 0.0f, 0.0f};
-    e.pid = seq_page(a.b, seq, pg0 + i, a.kv.pages, err);
-    if (e.pid >= 0) {
-      const size_t sc = (size_t)e.pid * a.kv.heads + head;
-      const float vs = fmaxf(a.kv.vs[sc], 0x1p-100f);
-      e.ks = a.scale * a.kv.ks[sc] * 1.4426950408889634f;
-      e.lv = log2f(vs);
-      e.rv = 1.0f / vs;
-    }
-    sm.pages[i] = e;
-  }
-
-  // Q fragments of rows g and g + 8, scaled by a power of two per row
-  uint32_t qf[DIM / 16][4];
-  float q_unit[2];
-  {
-    const T* q = static_cast<const T*>(a.q);
-#pragma unroll
-    for (int rr = 0; rr < 2; ++rr) {
-      const int r = r0 + g + 8 * rr;
-      const bool in = g + 8 * rr < nr;
-      const int t = r / a.group, hq = head * a.group + r - t * a.group;
-      const T* src = q + (long long)(sv.row0 + t) * a.q_token + (long long)hq * a.q_head;
-      float top = 0.0f;
-      // two passes over the row (the second is in cache): the largest element, then the values
-      if (in) {
-        for (int i = 0; i < DIM / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to_f(src[(i / 4) * 64 + c * 16 + 4 * (i % 4) + e])));
-      }
-      top = quad_max(top);
-      const Pow2 f = row_pow2(top);
-      const float down = f.down;
-      q_unit[rr] = f.up;
-#pragma unroll
-      for (int i = 0; i < DIM / 16; ++i) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[e] = in ? to_f(src[(i / 4) * 64 + c * 16 + 4 * (i % 4) + e]) * down : 0.0f;
-        qf[i][rr] = pack_f16(x[0], x[1]);
-        qf[i][2 + rr] = pack_f16(x[2], x[3]);
-      }
-    }
-  }
-  // the keys rows g and g + 8 see: [lo, hi)
-  int see_lo[2], see_hi[2];
-#pragma unroll
-  for (int rr = 0; rr < 2; ++rr) {
-    const int pos = pos0 + (r0 + g + 8 * rr) / a.group;
-    see_hi[rr] = a.causal ? min(sv.len, pos + 1) : sv.len;
-    see_lo[rr] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (pos < 0) see_hi[rr] = 0;
-  }
-  // units that every row of the tile sees whole
-  const int all_lo = a.window > 0 ? max(0, pos0 + t_last - a.window + 1) : 0;
-  const int all_hi = pos0 + t_first < 0 ? 0 : a.causal ? min(sv.len, pos0 + t_first + 1) : sv.len;
-
-  float o[NT][4];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  for (int i = threadIdx.x; i < npg; i += blockDim.x) sm.pages[i].pid = seq_page(a.b, seq, pg0 + i, a.kv.pages, err);
   __syncthreads();
 
   uint4 kc[2][KR];
   uint32_t vr[4][VW];
   auto place = [&](int u) -> size_t {  // byte offset of the unit's first key, this head
-    const PageEntry& e = sm.pages[((u * kUnit) >> lg) - pg0];
+    const int pid = sm.pages[((u * kUnit) >> lg) - pg0].pid;
     const int slot = (u * kUnit) & (a.kv.page - 1);
-    return (((size_t)max(e.pid, 0) * a.kv.heads + head) * a.kv.page + slot) * DIM;
+    return (((size_t)max(pid, 0) * a.kv.heads + head) * a.kv.page + slot) * DIM;
   };
   auto load_k = [&](int u) {
     const int8_t* b = a.kv.k + place(u) + g * DIM + c * 16;
@@ -220,28 +159,96 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
       }
     }
   };
-
   int u = ub + warp;
-  if (u < ue) {
+  if (u < ue) {  // on their way while the scales and Q are
     load_k(u);
     load_v(u);
   }
+  for (int i = threadIdx.x; i < npg; i += blockDim.x) {
+    PageEntry e = {sm.pages[i].pid, 0.0f, 0.0f, 0.0f};
+    if (e.pid >= 0) {
+      const size_t sc = (size_t)e.pid * a.kv.heads + head;
+      const float vs = fmaxf(a.kv.vs[sc], 0x1p-100f);
+      e.ks = a.scale * a.kv.ks[sc] * 1.4426950408889634f;
+      e.lv = log2f(vs);
+      e.rv = 1.0f / vs;
+    }
+    sm.pages[i] = e;  // by the thread that wrote its pid
+  }
+
+  // Q fragments of rows g and g + 8, scaled by a power of two per row; every warp reads the rows for
+  // their maxima and writes its share of the fragments
+  float q_unit[2];
+  {
+    const T* q = static_cast<const T*>(a.q);
+    uint32_t f[(DIM / 16 + kWarps - 1) / kWarps][4];
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+      const int r = r0 + g + 8 * rr;
+      const bool in = g + 8 * rr < nr;
+      const int t = r / a.group, hq = head * a.group + r - t * a.group;
+      const T* src = q + (long long)(sv.row0 + t) * a.q_token + (long long)hq * a.q_head + c * 16;
+      float top = 0.0f;
+      if (in) {
+#pragma unroll
+        for (int i = 0; i < DIM / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to_f(src[(i / 4) * 64 + 4 * (i % 4) + e])));
+      }
+      top = quad_max(top);
+      const Pow2 w = row_pow2(top);
+      q_unit[rr] = w.up;
+#pragma unroll
+      for (int k = 0; k < DIM / 16 / kWarps; ++k) {
+        const int i = warp + k * kWarps;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = in ? to_f(src[(i / 4) * 64 + 4 * (i % 4) + e]) * w.down : 0.0f;
+        f[k][rr] = pack_f16(x[0], x[1]);
+        f[k][2 + rr] = pack_f16(x[2], x[3]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < DIM / 16 / kWarps; ++k)
+      sm.q[warp + k * kWarps][lane] = make_uint4(f[k][0], f[k][1], f[k][2], f[k][3]);
+  }
+  // the keys rows g and g + 8 see: [lo, hi)
+  int see_lo[2], see_hi[2];
+#pragma unroll
+  for (int rr = 0; rr < 2; ++rr) {
+    const int pos = pos0 + (r0 + g + 8 * rr) / a.group;
+    see_hi[rr] = a.causal ? min(sv.len, pos + 1) : sv.len;
+    see_lo[rr] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    if (pos < 0) see_hi[rr] = 0;
+  }
+  // units that every row of the tile sees whole
+  const int all_lo = a.window > 0 ? max(0, pos0 + t_last - a.window + 1) : 0;
+  const int all_hi = pos0 + t_first < 0 ? 0 : a.causal ? min(sv.len, pos0 + t_first + 1) : sv.len;
+
+  float o[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  __syncthreads();
+
   for (; u < ue; u += kWarps) {
     const PageEntry e = sm.pages[((u * kUnit) >> lg) - pg0];
     // S: two n-tiles of 8 keys
     float s[2][4] = {};
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int r = 0; r < KR; ++r) {
+      const uint32_t w[2][4] = {{kc[0][r].x, kc[0][r].y, kc[0][r].z, kc[0][r].w},
+                                {kc[1][r].x, kc[1][r].y, kc[1][r].z, kc[1][r].w}};
 #pragma unroll
-      for (int r = 0; r < KR; ++r) {
-        const uint32_t w[4] = {kc[t][r].x, kc[t][r].y, kc[t][r].z, kc[t][r].w};
+      for (int i = 0; i < 4; ++i) {
+        const uint4 q = sm.q[r * 4 + i][lane];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t x = w[i] ^ 0x80808080u;
-          const int ks = r * 4 + i;
-          mma_f16(s[t], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], f16_from_u8(x, 0x4140), f16_from_u8(x, 0x4342));
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t x = w[t][i] ^ 0x80808080u;
+          mma_f16(s[t], q.x, q.y, q.z, q.w, f16_from_u8(x, 0x4140), f16_from_u8(x, 0x4342));
         }
       }
+    }
     const bool more = u + kWarps < ue;
     if (more) load_k(u + kWarps);
     // scores in powers of two, masked where the unit crosses an edge of what some row sees
@@ -265,7 +272,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
     const float top1 = quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])));
     if (__any_sync(0xffffffffu, top0 > m[0] + kMost || top1 > m[1] + kMost)) {
       const float n0 = fmaxf(m[0], top0 - kTop), n1 = fmaxf(m[1], top1 - kTop);
-      const float b0 = m[0] == n0 ? 1.0f : exp2f(m[0] - n0), b1 = m[1] == n1 ? 1.0f : exp2f(m[1] - n1);
+      const float b0 = m[0] == n0 ? 1.0f : ex2(m[0] - n0), b1 = m[1] == n1 ? 1.0f : ex2(m[1] - n1);
       m[0] = n0, m[1] = n1;
       l[0] *= b0, l[1] *= b1;
 #pragma unroll
@@ -276,8 +283,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
     float w[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      w[t][0] = exp2f(s[t][0] - m0), w[t][1] = exp2f(s[t][1] - m0);
-      w[t][2] = exp2f(s[t][2] - m1), w[t][3] = exp2f(s[t][3] - m1);
+      w[t][0] = ex2(s[t][0] - m0), w[t][1] = ex2(s[t][1] - m0);
+      w[t][2] = ex2(s[t][2] - m1), w[t][3] = ex2(s[t][3] - m1);
     }
     l[0] = fmaf((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]), e.rv, l[0]);
     l[1] = fmaf((w[0][2] + w[0][3]) + (w[1][2] + w[1][3]), e.rv, l[1]);
@@ -362,21 +369,36 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_stream(const StreamArgs p,
   __syncthreads();
   if (!sm.last) return;
   __threadfence();
-  for (int i = threadIdx.x; i < nr * (DIM / 2); i += blockDim.x) {
-    const int r = i / (DIM / 2), d = 2 * (i % (DIM / 2));
+  constexpr int PL = DIM / 32;  // elements per lane
+  for (int r = warp; r < nr; r += kWarps) {  // a warp per row, 32 chunks at a time
     const int t = (r0 + r) / a.group, hq = head * a.group + (r0 + r) - t * a.group;
     const size_t at = ((size_t)(sv.row0 + t) * a.q_heads + hq) * p.splits;
-    float top = -INFINITY, x = 0.0f, y = 0.0f, sum = 0.0f;
-    for (int k = 0; k < nsplit; ++k) top = fmaxf(top, __ldcg(&p.part_ml[at + k]).x);
-    for (int k = 0; k < nsplit; ++k) {
-      const float2 ml = __ldcg(&p.part_ml[at + k]);
-      const float b = ml.x == top ? 1.0f : exp2f(ml.x - top);
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(p.part_o + (at + k) * DIM + d));
-      sum = fmaf(ml.y, b, sum), x = fmaf(v.x, b, x), y = fmaf(v.y, b, y);
+    float top = -INFINITY;
+    for (int k = lane; k < nsplit; k += 32) top = fmaxf(top, __ldcg(&p.part_ml[at + k]).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float x[PL] = {}, sum = 0.0f;
+    for (int k0 = 0; k0 < nsplit; k0 += 32) {
+      const int n = min(32, nsplit - k0);
+      const float2 ml = lane < n ? __ldcg(&p.part_ml[at + k0 + lane]) : make_float2(-INFINITY, 0.0f);
+      const float mine = lane < n ? (ml.x == top ? 1.0f : ex2(ml.x - top)) : 0.0f;
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) {
+        const float b = __shfl_sync(0xffffffffu, mine, k);
+        sum = fmaf(__shfl_sync(0xffffffffu, ml.y, k), b, sum);
+        const float* v = p.part_o + (at + k0 + k) * DIM + lane * PL;
+#pragma unroll
+        for (int e = 0; e < PL; e += 2) {
+          const float2 w = __ldcg(reinterpret_cast<const float2*>(v + e));
+          x[e] = fmaf(w.x, b, x[e]), x[e + 1] = fmaf(w.y, b, x[e + 1]);
+        }
+      }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    store2(out + (long long)(sv.row0 + t) * a.o_token + (long long)hq * a.o_head + d, x * inv, y * inv);
-    if (d == 0 && a.lse)
+    T* dst = out + (long long)(sv.row0 + t) * a.o_token + (long long)hq * a.o_head + lane * PL;
+#pragma unroll
+    for (int e = 0; e < PL; e += 2) store2(dst + e, x[e] * inv, x[e + 1] * inv);
+    if (lane == 0 && a.lse)
       a.lse[(long long)(sv.row0 + t) * a.q_heads + hq] =
           sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
   }

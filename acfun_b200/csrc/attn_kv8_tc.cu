@@ -115,11 +115,6 @@ __device__ __forceinline__ void tmem_ld16p(uint32_t t, float* r) {
       : "r"(t));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* r) {
   asm volatile(
