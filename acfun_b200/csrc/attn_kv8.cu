@@ -31,7 +31,8 @@ namespace acf {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kUnit = 16;          // keys per step of a warp
+constexpr int kUnit = 16;          // keys that share a page entry
+constexpr int kPair = 2;           // units per step of a warp: two chains to hide each other's latencies
 constexpr int kMaxPages = 1024;    // pages of one chunk (their scales are staged in shared memory)
 constexpr int kTickets = 1 << 16;
 
@@ -98,7 +99,7 @@ struct StreamSmem {
 
 // DIM / 64 runs of 16 bytes per key for K; DIM / 8 bytes per key for V.
 template <typename T, int DIM>
-__global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : 4) k_attn_stream(const StreamArgs p, unsigned* err) {
+__global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 : 4) k_attn_stream(const StreamArgs p, unsigned* err) {
   constexpr int KR = DIM / 64;          // 16-byte runs of a thread per key (K)
   constexpr int NT = DIM / 8;           // output n-tiles
   constexpr int VW = DIM / 32;          // 32-bit words of a thread per key (V)
@@ -128,38 +129,45 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : 4) k_attn_stream
   for (int i = threadIdx.x; i < npg; i += blockDim.x) sm.pages[i].pid = seq_page(a.b, seq, pg0 + i, a.kv.pages, err);
   __syncthreads();
 
-  uint4 kc[2][KR];
-  uint32_t vr[4][VW];
+  uint4 kc[kPair][2][KR];
+  uint32_t vr[kPair][4][VW];
+  const size_t head_at = (size_t)head * a.kv.page, page_step = (size_t)a.kv.heads * a.kv.page;
   auto place = [&](int u) -> size_t {  // byte offset of the unit's first key, this head
     const int pid = sm.pages[((u * kUnit) >> lg) - pg0].pid;
-    const int slot = (u * kUnit) & (a.kv.page - 1);
-    return (((size_t)max(pid, 0) * a.kv.heads + head) * a.kv.page + slot) * DIM;
+    return (max(pid, 0) * page_step + head_at + ((u * kUnit) & (a.kv.page - 1))) * DIM;
   };
+  // units from u on; past the chunk's end the last one again (masked below)
   auto load_k = [&](int u) {
-    const int8_t* b = a.kv.k + place(u) + g * DIM + c * 16;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int p = 0; p < kPair; ++p) {
+      const int8_t* b = a.kv.k + place(min(u + p, ue - 1)) + g * DIM + c * 16;
 #pragma unroll
-      for (int r = 0; r < KR; ++r) kc[t][r] = ldg16(b + t * 8 * DIM + r * 64);
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < KR; ++r) kc[p][t][r] = ldg16(b + t * 8 * DIM + r * 64);
+    }
   };
   auto load_v = [&](int u) {
-    const int8_t* b = a.kv.v + place(u) + g * (DIM / 8);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int8_t* s = b + (2 * c + (k & 1) + 8 * (k >> 1)) * DIM;
-      if constexpr (DIM == 64) {
-        const uint2 w = ldg8(s);
-        vr[k][0] = w.x, vr[k][1] = w.y;
-      } else {
+    for (int p = 0; p < kPair; ++p) {
+      const int8_t* b = a.kv.v + place(min(u + p, ue - 1)) + g * (DIM / 8) + 2 * c * DIM;
 #pragma unroll
-        for (int r = 0; r < VW / 4; ++r) {
-          const uint4 w = ldg16(s + 16 * r);
-          vr[k][4 * r] = w.x, vr[k][4 * r + 1] = w.y, vr[k][4 * r + 2] = w.z, vr[k][4 * r + 3] = w.w;
+      for (int k = 0; k < 4; ++k) {
+        const int8_t* s = b + ((k & 1) + 8 * (k >> 1)) * DIM;
+        if constexpr (DIM == 64) {
+          const uint2 w = ldg8(s);
+          vr[p][k][0] = w.x, vr[p][k][1] = w.y;
+        } else {
+#pragma unroll
+          for (int r = 0; r < VW / 4; ++r) {
+            const uint4 w = ldg16(s + 16 * r);
+            vr[p][k][4 * r] = w.x, vr[p][k][4 * r + 1] = w.y, vr[p][k][4 * r + 2] = w.z, vr[p][k][4 * r + 3] = w.w;
+          }
         }
       }
     }
   };
-  int u = ub + warp;
+  int u = ub + warp * kPair;
   if (u < ue) {  // on their way while the scales and Q are
     load_k(u);
     load_v(u);
@@ -231,47 +239,62 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : 4) k_attn_stream
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   __syncthreads();
 
-  for (; u < ue; u += kWarps) {
-    const PageEntry e = sm.pages[((u * kUnit) >> lg) - pg0];
-    // S: two n-tiles of 8 keys
-    float s[2][4] = {};
+  for (; u < ue; u += kWarps * kPair) {
+    // S: two n-tiles of 8 keys per unit
+    float s[kPair][2][4] = {};
 #pragma unroll
-    for (int r = 0; r < KR; ++r) {
-      const uint32_t w[2][4] = {{kc[0][r].x, kc[0][r].y, kc[0][r].z, kc[0][r].w},
-                                {kc[1][r].x, kc[1][r].y, kc[1][r].z, kc[1][r].w}};
+    for (int r = 0; r < KR; ++r)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint4 q = sm.q[r * 4 + i][lane];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t x = w[t][i] ^ 0x80808080u;
-          mma_f16(s[t], q.x, q.y, q.z, q.w, f16_from_u8(x, 0x4140), f16_from_u8(x, 0x4342));
-        }
+        for (int p = 0; p < kPair; ++p)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint4& k4 = kc[p][t][r];
+            const uint32_t x = (i == 0 ? k4.x : i == 1 ? k4.y : i == 2 ? k4.z : k4.w) ^ 0x80808080u;
+            mma_f16(s[p][t], q.x, q.y, q.z, q.w, f16_from_u8(x, 0x4140), f16_from_u8(x, 0x4342));
+          }
+      }
+    const bool more = u + kWarps * kPair < ue;
+    if (more) load_k(u + kWarps * kPair);
+    // scores in powers of two, masked where the step crosses an edge of what some row sees
+    const int k0 = u * kUnit;
+    float rv[kPair];
+    bool whole = k0 >= all_lo && k0 + kPair * kUnit <= all_hi && u + kPair <= ue;
+#pragma unroll
+    for (int p = 0; p < kPair; ++p) {
+      const PageEntry e = sm.pages[((min(u + p, ue - 1) * kUnit) >> lg) - pg0];
+      rv[p] = e.rv;
+      whole = whole && e.pid >= 0;
+      const float f0 = e.ks * q_unit[0], f1 = e.ks * q_unit[1], lv = e.pid >= 0 && u + p < ue ? e.lv : -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[p][t][0] = fmaf(s[p][t][0], f0, lv), s[p][t][1] = fmaf(s[p][t][1], f0, lv);
+        s[p][t][2] = fmaf(s[p][t][2], f1, lv), s[p][t][3] = fmaf(s[p][t][3], f1, lv);
       }
     }
-    const bool more = u + kWarps < ue;
-    if (more) load_k(u + kWarps);
-    // scores in powers of two, masked where the unit crosses an edge of what some row sees
-    const int k0 = u * kUnit;
-    const float f0 = e.ks * q_unit[0], f1 = e.ks * q_unit[1];
+    if (__builtin_expect(!whole, 0)) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t][0] = fmaf(s[t][0], f0, e.lv), s[t][1] = fmaf(s[t][1], f0, e.lv);
-      s[t][2] = fmaf(s[t][2], f1, e.lv), s[t][3] = fmaf(s[t][3], f1, e.lv);
+      for (int p = 0; p < kPair; ++p)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = k0 + p * kUnit + 8 * t + 2 * c + (i & 1);
+            if (key < see_lo[i >> 1] || key >= see_hi[i >> 1]) s[p][t][i] = -INFINITY;
+          }
     }
-    if (k0 < all_lo || k0 + kUnit > all_hi || e.pid < 0) {
+    float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = k0 + 8 * t + 2 * c + (i & 1);
-          if (key < see_lo[i >> 1] || key >= see_hi[i >> 1] || e.pid < 0) s[t][i] = -INFINITY;
-        }
+    for (int p = 0; p < kPair; ++p) {
+      top0 = fmaxf(top0, fmaxf(fmaxf(s[p][0][0], s[p][0][1]), fmaxf(s[p][1][0], s[p][1][1])));
+      top1 = fmaxf(top1, fmaxf(fmaxf(s[p][0][2], s[p][0][3]), fmaxf(s[p][1][2], s[p][1][3])));
     }
-    const float top0 = quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])));
-    const float top1 = quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])));
-    if (__any_sync(0xffffffffu, top0 > m[0] + kMost || top1 > m[1] + kMost)) {
-      const float n0 = fmaxf(m[0], top0 - kTop), n1 = fmaxf(m[1], top1 - kTop);
+    // a thread's own scores say whether an offset has to move; the rows' maxima are looked up only then
+    if (__builtin_expect(__any_sync(0xffffffffu, top0 > m[0] + kMost || top1 > m[1] + kMost), 0)) {
+      top0 = quad_max(top0), top1 = quad_max(top1);
+      const float n0 = top0 > m[0] + kMost ? top0 - kTop : m[0], n1 = top1 > m[1] + kMost ? top1 - kTop : m[1];
       const float b0 = m[0] == n0 ? 1.0f : ex2(m[0] - n0), b1 = m[1] == n1 ? 1.0f : ex2(m[1] - n1);
       m[0] = n0, m[1] = n1;
       l[0] *= b0, l[1] *= b1;
@@ -280,29 +303,32 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : 4) k_attn_stream
     }
     // a row that has seen nothing yet has m = -inf and only -inf scores
     const float m0 = m[0] == -INFINITY ? 0.0f : m[0], m1 = m[1] == -INFINITY ? 0.0f : m[1];
-    float w[2][4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      w[t][0] = ex2(s[t][0] - m0), w[t][1] = ex2(s[t][1] - m0);
-      w[t][2] = ex2(s[t][2] - m1), w[t][3] = ex2(s[t][3] - m1);
-    }
-    l[0] = fmaf((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]), e.rv, l[0]);
-    l[1] = fmaf((w[0][2] + w[0][3]) + (w[1][2] + w[1][3]), e.rv, l[1]);
-    const uint32_t a0 = pack_f16(w[0][0], w[0][1]), a1 = pack_f16(w[0][2], w[0][3]);
-    const uint32_t a2 = pack_f16(w[1][0], w[1][1]), a3 = pack_f16(w[1][2], w[1][3]);
-    // O: n-tile j holds elements (lane / 4) * DIM / 8 + j of the head
+    for (int p = 0; p < kPair; ++p) {
+      float w[2][4];
 #pragma unroll
-    for (int i = 0; i < VW; ++i) {
-      const uint32_t x0 = vr[0][i] ^ 0x80808080u, x1 = vr[1][i] ^ 0x80808080u;
-      const uint32_t x2 = vr[2][i] ^ 0x80808080u, x3 = vr[3][i] ^ 0x80808080u;
-      const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
-      const uint32_t s0 = __byte_perm(x2, x3, 0x5140), s1 = __byte_perm(x2, x3, 0x7362);
-      mma_f16(o[4 * i], a0, a1, a2, a3, f16_from_u8(p0, 0x4140), f16_from_u8(s0, 0x4140));
-      mma_f16(o[4 * i + 1], a0, a1, a2, a3, f16_from_u8(p0, 0x4342), f16_from_u8(s0, 0x4342));
-      mma_f16(o[4 * i + 2], a0, a1, a2, a3, f16_from_u8(p1, 0x4140), f16_from_u8(s1, 0x4140));
-      mma_f16(o[4 * i + 3], a0, a1, a2, a3, f16_from_u8(p1, 0x4342), f16_from_u8(s1, 0x4342));
+      for (int t = 0; t < 2; ++t) {
+        w[t][0] = ex2(s[p][t][0] - m0), w[t][1] = ex2(s[p][t][1] - m0);
+        w[t][2] = ex2(s[p][t][2] - m1), w[t][3] = ex2(s[p][t][3] - m1);
+      }
+      l[0] = fmaf((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]), rv[p], l[0]);
+      l[1] = fmaf((w[0][2] + w[0][3]) + (w[1][2] + w[1][3]), rv[p], l[1]);
+      const uint32_t a0 = pack_f16(w[0][0], w[0][1]), a1 = pack_f16(w[0][2], w[0][3]);
+      const uint32_t a2 = pack_f16(w[1][0], w[1][1]), a3 = pack_f16(w[1][2], w[1][3]);
+      // O: n-tile j holds elements (lane / 4) * DIM / 8 + j of the head
+#pragma unroll
+      for (int i = 0; i < VW; ++i) {
+        const uint32_t x0 = vr[p][0][i] ^ 0x80808080u, x1 = vr[p][1][i] ^ 0x80808080u;
+        const uint32_t x2 = vr[p][2][i] ^ 0x80808080u, x3 = vr[p][3][i] ^ 0x80808080u;
+        const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
+        const uint32_t s0 = __byte_perm(x2, x3, 0x5140), s1 = __byte_perm(x2, x3, 0x7362);
+        mma_f16(o[4 * i], a0, a1, a2, a3, f16_from_u8(p0, 0x4140), f16_from_u8(s0, 0x4140));
+        mma_f16(o[4 * i + 1], a0, a1, a2, a3, f16_from_u8(p0, 0x4342), f16_from_u8(s0, 0x4342));
+        mma_f16(o[4 * i + 2], a0, a1, a2, a3, f16_from_u8(p1, 0x4140), f16_from_u8(s1, 0x4140));
+        mma_f16(o[4 * i + 3], a0, a1, a2, a3, f16_from_u8(p1, 0x4342), f16_from_u8(s1, 0x4342));
+      }
     }
-    if (more) load_v(u + kWarps);
+    if (more) load_v(u + kWarps * kPair);
   }
 
   // ---- the four warps' parts joined
@@ -447,7 +473,7 @@ bool stream_launch(Call& c, const AttnArgs& a) {
   const long long want = std::max<long long>(1, slots / std::max<long long>(1, work));
   long long chunk = (a.b.max_len + want - 1) / want;
   if (a.b.seqs > 1) chunk = std::min<long long>(chunk, 1024);
-  chunk = std::max<long long>(chunk, kUnit * kWarps);
+  chunk = std::max<long long>(chunk, kUnit * kPair * kWarps);
   chunk = std::min<long long>((chunk + kUnit - 1) / kUnit * kUnit, (long long)(kMaxPages - 1) * a.kv.page);
   p.chunk = (int)chunk;
   p.splits = (int)((a.b.max_len + 2 * kUnit + chunk - 1) / chunk);
