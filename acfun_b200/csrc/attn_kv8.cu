@@ -1,6 +1,5 @@
 // attn_kv8.cu — attention over the int8 cache (acfun_kv8_attention): the entry point and the
-// streaming kernel, which reads codes straight from global memory into matrix-instruction
-// fragments.  It takes any shape; attention with few rows per cache head (decode steps, drafts)
+// streaming kernel, whose warps turn codes straight into matrix-instruction fragments.  It takes any shape; attention with few rows per cache head (decode steps, drafts)
 // is bound by the codes it reads, and that is what it is built for.
 //
 // Rows: the new tokens of a sequence times the query heads that share a cache head, row = token *
@@ -20,7 +19,8 @@
 // Fragments.  K is the B operand of m16n8k16 with its contraction index (the element of a head)
 // permuted so that a thread's share of a key is 16 consecutive bytes; V is the B operand with its
 // column index permuted so that a thread's share of each of its four keys is 16 consecutive bytes
-// (8 when dim is 64).  Both come by 16-byte loads, whole sectors, with no staging.
+// (8 when dim is 64).  The codes pass through a ring in shared memory of two steps of 32 keys per
+// warp, copied asynchronously; nothing is shared between warps.
 #include <math.h>
 
 #include <algorithm>
@@ -61,19 +61,6 @@ __device__ __forceinline__ float quad_sum(float x) {
   x += __shfl_xor_sync(0xffffffffu, x, 1);
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
-
 // What a page needs in the loop: its place, and its scales in the forms used.
 struct PageEntry {
   int pid;          // -1: out of range (reported), its keys are not seen
@@ -87,6 +74,31 @@ __device__ __forceinline__ void store2(T* p, float a, float b) {
   p[1] = from_f<T>(b);
 }
 
+// A warp's codes on their way: two steps, each kPair units of 16 keys of K and V.  16-byte chunk ch
+// of a row is kept at chunk_at(row, ch), so that the fragment reads below (two rows x 4 chunks of K,
+// four alternate rows x 2 chunks of V at a time) meet no bank twice.
+template <int DIM>
+struct Ring {
+  uint8_t kv[2][2][kPair * kUnit * DIM];  // [step][K, V]
+};
+template <int DIM>
+__device__ __forceinline__ int chunk_at(int row, int ch) {
+  if constexpr (DIM == 64) {
+    const int unit = ((row & 1) * 4 + ch) ^ (row & 6);
+    return (row >> 1) * 128 + unit * 16;
+  } else {
+    return row * DIM + (ch >> 3) * 128 + (((ch & 7) ^ (row & 6) ^ ((row & 1) << 2)) << 4);
+  }
+}
+__device__ __forceinline__ void cp16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dev::smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <int DIM>
 struct StreamSmem {
   PageEntry pages[kMaxPages];
@@ -94,7 +106,10 @@ struct StreamSmem {
   float row_ml[16][2];
   int last;
   uint4 q[DIM / 16][32];  // Q fragments, the same for the four warps
-  float o[kWarps][16][DIM + 4];
+  union {
+    Ring<DIM> ring[kWarps];
+    float o[kWarps][16][DIM + 4];
+  };
 };
 
 // DIM / 64 runs of 16 bytes per key for K; DIM / 8 bytes per key for V.
@@ -129,49 +144,32 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
   for (int i = threadIdx.x; i < npg; i += blockDim.x) sm.pages[i].pid = seq_page(a.b, seq, pg0 + i, a.kv.pages, err);
   __syncthreads();
 
-  uint4 kc[kPair][2][KR];
-  uint32_t vr[kPair][4][VW];
   const size_t head_at = (size_t)head * a.kv.page, page_step = (size_t)a.kv.heads * a.kv.page;
-  auto place = [&](int u) -> size_t {  // byte offset of the unit's first key, this head
-    const int pid = sm.pages[((u * kUnit) >> lg) - pg0].pid;
-    return (max(pid, 0) * page_step + head_at + ((u * kUnit) & (a.kv.page - 1))) * DIM;
-  };
-  // units from u on; past the chunk's end the last one again (masked below)
-  auto load_k = [&](int u) {
+  Ring<DIM>& ring = sm.ring[warp];
+  // Requests the units from u on as step `at`; past the chunk's end the last one again (masked below).
+  auto request = [&](int u, int at) {
+    constexpr int CH = DIM / 16, RPP = 32 / CH;  // chunks per row, rows per pass
+    const int row0 = lane / CH, ch = lane % CH;
 #pragma unroll
     for (int p = 0; p < kPair; ++p) {
-      const int8_t* b = a.kv.k + place(min(u + p, ue - 1)) + g * DIM + c * 16;
+      const int key = min(u + p, ue - 1) * kUnit;
+      const int pid = sm.pages[(key >> lg) - pg0].pid;
+      const size_t from = (max(pid, 0) * page_step + head_at + (key & (a.kv.page - 1)) + row0) * DIM + ch * 16;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < KR; ++r) kc[p][t][r] = ldg16(b + t * 8 * DIM + r * 64);
-    }
-  };
-  auto load_v = [&](int u) {
-#pragma unroll
-    for (int p = 0; p < kPair; ++p) {
-      const int8_t* b = a.kv.v + place(min(u + p, ue - 1)) + g * (DIM / 8) + 2 * c * DIM;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int8_t* s = b + ((k & 1) + 8 * (k >> 1)) * DIM;
-        if constexpr (DIM == 64) {
-          const uint2 w = ldg8(s);
-          vr[p][k][0] = w.x, vr[p][k][1] = w.y;
-        } else {
-#pragma unroll
-          for (int r = 0; r < VW / 4; ++r) {
-            const uint4 w = ldg16(s + 16 * r);
-            vr[p][k][4 * r] = w.x, vr[p][k][4 * r + 1] = w.y, vr[p][k][4 * r + 2] = w.z, vr[p][k][4 * r + 3] = w.w;
-          }
-        }
+      for (int r = 0; r < kUnit; r += RPP) {
+        const int to = chunk_at<DIM>(p * kUnit + r + row0, ch);
+        cp16(&ring.kv[at][0][to], a.kv.k + from + r * DIM);
+        cp16(&ring.kv[at][1][to], a.kv.v + from + r * DIM);
       }
     }
   };
   int u = ub + warp * kPair;
-  if (u < ue) {  // on their way while the scales and Q are
-    load_k(u);
-    load_v(u);
-  }
+  constexpr int kStride = kWarps * kPair;
+  // two steps on their way while the scales and Q are
+  if (u < ue) request(u, 0);
+  cp_commit();
+  if (u + kStride < ue) request(u + kStride, 1);
+  cp_commit();
   for (int i = threadIdx.x; i < npg; i += blockDim.x) {
     PageEntry e = {sm.pages[i].pid, 0.0f, 0.0f, 0.0f};
     if (e.pid >= 0) {
@@ -239,11 +237,20 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   __syncthreads();
 
-  for (; u < ue; u += kWarps * kPair) {
+  for (int at = 0; u < ue; u += kStride, at ^= 1) {
+    cp_wait<1>();
+    __syncwarp();
+    const uint8_t *ks = ring.kv[at][0], *vs = ring.kv[at][1];
     // S: two n-tiles of 8 keys per unit
     float s[kPair][2][4] = {};
 #pragma unroll
-    for (int r = 0; r < KR; ++r)
+    for (int r = 0; r < KR; ++r) {
+      uint4 kc[kPair][2];
+#pragma unroll
+      for (int p = 0; p < kPair; ++p)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          kc[p][t] = *reinterpret_cast<const uint4*>(ks + chunk_at<DIM>(p * kUnit + t * 8 + g, r * 4 + c));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint4 q = sm.q[r * 4 + i][lane];
@@ -251,13 +258,12 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
         for (int p = 0; p < kPair; ++p)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const uint4& k4 = kc[p][t][r];
+            const uint4& k4 = kc[p][t];
             const uint32_t x = (i == 0 ? k4.x : i == 1 ? k4.y : i == 2 ? k4.z : k4.w) ^ 0x80808080u;
             mma_f16(s[p][t], q.x, q.y, q.z, q.w, f16_from_u8(x, 0x4140), f16_from_u8(x, 0x4342));
           }
       }
-    const bool more = u + kWarps * kPair < ue;
-    if (more) load_k(u + kWarps * kPair);
+    }
     // scores in powers of two, masked where the step crosses an edge of what some row sees
     const int k0 = u * kUnit;
     float rv[kPair];
@@ -315,11 +321,26 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
       l[1] = fmaf((w[0][2] + w[0][3]) + (w[1][2] + w[1][3]), rv[p], l[1]);
       const uint32_t a0 = pack_f16(w[0][0], w[0][1]), a1 = pack_f16(w[0][2], w[0][3]);
       const uint32_t a2 = pack_f16(w[1][0], w[1][1]), a3 = pack_f16(w[1][2], w[1][3]);
+      uint32_t vr[4][VW];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = p * kUnit + 2 * c + (k & 1) + 8 * (k >> 1);
+        if constexpr (DIM == 64) {
+          const uint2 w2 = *reinterpret_cast<const uint2*>(vs + chunk_at<DIM>(row, g >> 1) + 8 * (g & 1));
+          vr[k][0] = w2.x, vr[k][1] = w2.y;
+        } else {
+#pragma unroll
+          for (int r = 0; r < VW / 4; ++r) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(vs + chunk_at<DIM>(row, g * (VW / 4) + r));
+            vr[k][4 * r] = w4.x, vr[k][4 * r + 1] = w4.y, vr[k][4 * r + 2] = w4.z, vr[k][4 * r + 3] = w4.w;
+          }
+        }
+      }
       // O: n-tile j holds elements (lane / 4) * DIM / 8 + j of the head
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
-        const uint32_t x0 = vr[p][0][i] ^ 0x80808080u, x1 = vr[p][1][i] ^ 0x80808080u;
-        const uint32_t x2 = vr[p][2][i] ^ 0x80808080u, x3 = vr[p][3][i] ^ 0x80808080u;
+        const uint32_t x0 = vr[0][i] ^ 0x80808080u, x1 = vr[1][i] ^ 0x80808080u;
+        const uint32_t x2 = vr[2][i] ^ 0x80808080u, x3 = vr[3][i] ^ 0x80808080u;
         const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
         const uint32_t s0 = __byte_perm(x2, x3, 0x5140), s1 = __byte_perm(x2, x3, 0x7362);
         mma_f16(o[4 * i], a0, a1, a2, a3, f16_from_u8(p0, 0x4140), f16_from_u8(s0, 0x4140));
@@ -328,16 +349,19 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
         mma_f16(o[4 * i + 3], a0, a1, a2, a3, f16_from_u8(p1, 0x4342), f16_from_u8(s1, 0x4342));
       }
     }
-    if (more) load_v(u + kWarps * kPair);
+    __syncwarp();
+    if (u + 2 * kStride < ue) request(u + 2 * kStride, at);
+    cp_commit();
   }
+  cp_wait<0>();
 
-  // ---- the four warps' parts joined
+  // ---- the four warps' parts joined (the outputs take the place of the codes)
   l[0] = quad_sum(l[0]), l[1] = quad_sum(l[1]);
   if (c == 0) {
     sm.ml[warp][g] = make_float2(m[0], l[0]);
     sm.ml[warp][g + 8] = make_float2(m[1], l[1]);
   }
-  __syncthreads();
+  __syncthreads();  // also: no warp reads codes any more
 #pragma unroll
   for (int rr = 0; rr < 2; ++rr) {
     const int r = g + 8 * rr;
