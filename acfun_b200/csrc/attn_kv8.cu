@@ -33,7 +33,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;          // keys that share a page entry
 constexpr int kPair = 2;           // units per step of a warp: two chains to hide each other's latencies
-constexpr int kMaxPages = 1024;    // pages of one chunk (their scales are staged in shared memory)
+constexpr int kMaxPages = 1024;    // most pages of one chunk (their scales are staged in shared memory)
 constexpr int kTickets = 1 << 16;
 
 struct StreamArgs {
@@ -62,7 +62,7 @@ __device__ __forceinline__ float quad_sum(float x) {
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
 // What a page needs in the loop: its place, and its scales in the forms used.
-struct PageEntry {
+struct __align__(16) PageEntry {
   int pid;          // -1: out of range (reported), its keys are not seen
   float ks;         // scale * k scale * log2 e
   float lv, rv;     // log2 and reciprocal of the v scale
@@ -101,7 +101,6 @@ __device__ __forceinline__ void cp_wait() {
 
 template <int DIM>
 struct StreamSmem {
-  PageEntry pages[kMaxPages];
   float2 ml[kWarps][16];
   float row_ml[16][2];
   int last;
@@ -110,6 +109,7 @@ struct StreamSmem {
     Ring<DIM> ring[kWarps];
     float o[kWarps][16][DIM + 4];
   };
+  PageEntry pages[1];  // as many as a chunk can touch: the launch sizes the block's memory by them
 };
 
 // DIM / 64 runs of 16 bytes per key for K; DIM / 8 bytes per key for V.
@@ -472,13 +472,13 @@ unsigned* tickets_of(int device) {
 
 template <typename T, int DIM>
 bool stream_launch(Call& c, const AttnArgs& a) {
-  const int smem = (int)sizeof(StreamSmem<DIM>);
-  static int per_sm[64] = {};
+  constexpr int kBase = (int)sizeof(StreamSmem<DIM>), kMost = kBase + kMaxPages * (int)sizeof(PageEntry);
+  static int per_sm[64] = {};  // blocks per SM with few pages, which is the case where it counts
   const int dv = current_device() & 63;
   if (!per_sm[dv]) {
     int n = 0;
-    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_stream<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) ||
-        !ACF_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn_stream<T, DIM>, kWarps * 32, smem)))
+    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_stream<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost)) ||
+        !ACF_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn_stream<T, DIM>, kWarps * 32, kBase + 1024)))
       return false;
     per_sm[dv] = std::max(1, n);
   }
@@ -519,6 +519,7 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     }
     if (!c.ok() || !p.tickets) return false;
   }
+  const int smem = kBase + (int)std::min<long long>(chunk / a.kv.page + 2, kMaxPages) * (int)sizeof(PageEntry);
   k_attn_stream<T, DIM><<<dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), kWarps * 32, smem, c.stream()>>>(p, c.err());
   return c.launched("k_attn_stream");
 }
