@@ -3,11 +3,11 @@
 // is bound by the codes it reads, and that is what it is built for.
 //
 // Rows: the new tokens of a sequence times the query heads that share a cache head, row = token *
-// group + head, in tiles of 16.  A block of four warps takes one (sequence, cache head, row tile,
-// chunk of keys); its warps take units of 16 keys in turn, each with its own running maximum, sum
-// and output, which are joined in shared memory at the end.  A long sequence is split over
-// blocks; the last of them to finish joins their parts in the order of the chunks, so the result
-// does not depend on who was last.
+// group + head, in tiles of 8, 16 or 32.  A block of four warps takes one (sequence, cache head, row
+// tile, chunk of keys); its warps take 32 keys in turn, each with its own running offset, sum and
+// output, which are joined in shared memory at the end.  A long sequence is split over blocks; the
+// last of them to finish joins their parts in the order of the chunks, so the result does not
+// depend on who was last.
 //
 // Mathematics.  With q scaled per row by a power of two to fp16 range (exact for what matters:
 // 11 bits below the row's largest element), codes c exact in fp16, S = q.c_k in fp32,
@@ -16,11 +16,15 @@
 // The V scale rides in the exponent, so O needs no per-page scaling and w stays within fp16 range
 // whatever the scales are; m moves only when a weight would pass 2^15.
 //
-// Fragments.  K is the B operand of m16n8k16 with its contraction index (the element of a head)
-// permuted so that a thread's share of a key is 16 consecutive bytes; V is the B operand with its
-// column index permuted so that a thread's share of each of its four keys is 16 consecutive bytes
-// (8 when dim is 64).  The codes pass through a ring in shared memory of two steps of 32 keys per
-// warp, copied asynchronously; nothing is shared between warps.
+// Fragments.  The products are transposed, S^T = K Q^T and O^T = V^T w^T, so that keys and elements
+// take the 16 places of m16n8k16 and the rows the 8: a decode step's few rows leave none of them
+// idle (with the rows in the 16 places, half of the products were of nothing, and the board's
+// power limit, which this kernel reaches, made that time).  K is the A operand with its contraction
+// index (the element of a head) permuted so that a thread's share of a key is 16 consecutive bytes;
+// V^T is the A operand with its row index permuted so that a thread's share of each of its four keys
+// is 16 consecutive bytes (8 when dim is 64); the weights change from C to B operand by movmatrix.
+// The codes pass through a ring in shared memory of two steps of 32 keys per warp, copied
+// asynchronously; nothing is shared between warps.
 #include <math.h>
 
 #include <algorithm>
@@ -53,13 +57,21 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+// over the eight lanes that hold the same rows
+__device__ __forceinline__ float rows_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+__device__ __forceinline__ float rows_sum(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x + __shfl_xor_sync(0xffffffffu, x, 16);
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // of an 8 x 8 matrix of 16-bit elements
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 // What a page needs in the loop: its place, and its scales in the forms used.
 struct __align__(16) PageEntry {
@@ -78,7 +90,7 @@ __device__ __forceinline__ void store2(T* p, float a, float b) {
 // of a row is kept at chunk_at(row, ch), so that the fragment reads below (two rows x 4 chunks of K,
 // four alternate rows x 2 chunks of V at a time) meet no bank twice.
 template <int DIM>
-struct Ring {
+struct alignas(128) Ring {
   uint8_t kv[2][2][kPair * kUnit * DIM];  // [step][K, V]
 };
 template <int DIM>
@@ -99,35 +111,39 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <int DIM>
+template <int DIM, int R8>
 struct StreamSmem {
-  float2 ml[kWarps][16];
-  float row_ml[16][2];
+  float2 ml[kWarps][8 * R8];
+  float row_ml[8 * R8][2];
   int last;
-  uint4 q[DIM / 16][32];  // Q fragments, the same for the four warps
+  uint2 q[R8 > 1 ? DIM / 16 : 1][R8][32];  // Q fragments, the same for the four warps
   union {
     Ring<DIM> ring[kWarps];
-    float o[kWarps][16][DIM + 4];
+    float o[kWarps][8 * R8][DIM + 4];
   };
   PageEntry pages[1];  // as many as a chunk can touch: the launch sizes the block's memory by them
 };
+static_assert(alignof(StreamSmem<64, 1>) == 128 && alignof(Ring<64>) == 128 && sizeof(Ring<64>) % 128 == 0,
+              "16-byte copies into the ring");
 
 // DIM / 64 runs of 16 bytes per key for K; DIM / 8 bytes per key for V.
-template <typename T, int DIM>
-__global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 : 4) k_attn_stream(const StreamArgs p, unsigned* err) {
+template <typename T, int DIM, int R8>
+__global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_stream(const StreamArgs p, unsigned* err) {
   constexpr int KR = DIM / 64;          // 16-byte runs of a thread per key (K)
-  constexpr int NT = DIM / 8;           // output n-tiles
+  constexpr int MT = DIM / 16;          // output m-tiles
   constexpr int VW = DIM / 32;          // 32-bit words of a thread per key (V)
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  StreamSmem<DIM>& sm = *reinterpret_cast<StreamSmem<DIM>*>(smem_raw);
+  constexpr int RT = 8 * R8;            // rows of a tile
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  using Smem = StreamSmem<DIM, R8>;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const AttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int head = blockIdx.x % a.kv.heads, rt = blockIdx.x / a.kv.heads, seq = blockIdx.y, chunk_i = blockIdx.z;
   const SeqView sv = seq_view(a.b, seq, err);
   const int rows = sv.n * a.group;
-  const int r0 = rt * 16;
+  const int r0 = rt * RT;
   if (r0 >= rows) return;
-  const int nr = min(16, rows - r0);
+  const int nr = min(RT, rows - r0);
   const int t_first = r0 / a.group, t_last = (r0 + nr - 1) / a.group;
   const int pos0 = sv.len - sv.n;  // position of new token 0 (negative: it sees nothing)
   const KeyRange kr = key_range(a, sv, r0, nr, kUnit);
@@ -182,16 +198,16 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
     sm.pages[i] = e;  // by the thread that wrote its pid
   }
 
-  // Q fragments of rows g and g + 8, scaled by a power of two per row; every warp reads the rows for
-  // their maxima and writes its share of the fragments
-  float q_unit[2];
+  // Q fragments of row g of each eight, scaled by a power of two per row.  With one eight they stay in
+  // registers; with more, every warp reads the rows for their maxima and writes its share.
+  uint2 qf[DIM / 16];
+  float q_unit[R8][2];  // of rows 2 c, 2 c + 1 of each eight
   {
     const T* q = static_cast<const T*>(a.q);
-    uint32_t f[(DIM / 16 + kWarps - 1) / kWarps][4];
 #pragma unroll
-    for (int rr = 0; rr < 2; ++rr) {
-      const int r = r0 + g + 8 * rr;
-      const bool in = g + 8 * rr < nr;
+    for (int n = 0; n < R8; ++n) {
+      const int r = r0 + 8 * n + g;
+      const bool in = 8 * n + g < nr;
       const int t = r / a.group, hq = head * a.group + r - t * a.group;
       const T* src = q + (long long)(sv.row0 + t) * a.q_token + (long long)hq * a.q_head + c * 16;
       float top = 0.0f;
@@ -201,48 +217,56 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to_f(src[(i / 4) * 64 + 4 * (i % 4) + e])));
       }
-      top = quad_max(top);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const Pow2 w = row_pow2(top);
-      q_unit[rr] = w.up;
 #pragma unroll
-      for (int k = 0; k < DIM / 16 / kWarps; ++k) {
-        const int i = warp + k * kWarps;
+      for (int i = 0; i < DIM / 16; ++i) {
+        if (R8 > 1 && i % kWarps != warp) continue;
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = in ? to_f(src[(i / 4) * 64 + 4 * (i % 4) + e]) * w.down : 0.0f;
-        f[k][rr] = pack_f16(x[0], x[1]);
-        f[k][2 + rr] = pack_f16(x[2], x[3]);
+        qf[i] = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
+        if constexpr (R8 > 1) sm.q[i][n][lane] = qf[i];
       }
+      q_unit[n][0] = __shfl_sync(0xffffffffu, w.up, 8 * c);
+      q_unit[n][1] = __shfl_sync(0xffffffffu, w.up, 8 * c + 4);
     }
-#pragma unroll
-    for (int k = 0; k < DIM / 16 / kWarps; ++k)
-      sm.q[warp + k * kWarps][lane] = make_uint4(f[k][0], f[k][1], f[k][2], f[k][3]);
   }
-  // the keys rows g and g + 8 see: [lo, hi)
-  int see_lo[2], see_hi[2];
+  // the keys rows 2 c, 2 c + 1 of each eight see: [lo, hi)
+  int see_lo[R8][2], see_hi[R8][2];
 #pragma unroll
-  for (int rr = 0; rr < 2; ++rr) {
-    const int pos = pos0 + (r0 + g + 8 * rr) / a.group;
-    see_hi[rr] = a.causal ? min(sv.len, pos + 1) : sv.len;
-    see_lo[rr] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (pos < 0) see_hi[rr] = 0;
-  }
+  for (int n = 0; n < R8; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int pos = pos0 + (r0 + 8 * n + 2 * c + i) / a.group;
+      see_hi[n][i] = a.causal ? min(sv.len, pos + 1) : sv.len;
+      see_lo[n][i] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      if (pos < 0) see_hi[n][i] = 0;
+    }
   // units that every row of the tile sees whole
   const int all_lo = a.window > 0 ? max(0, pos0 + t_last - a.window + 1) : 0;
   const int all_hi = pos0 + t_first < 0 ? 0 : a.causal ? min(sv.len, pos0 + t_first + 1) : sv.len;
 
-  float o[NT][4];
+  float o[MT][R8][4];
+  float m[R8][2], l[R8][2];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  for (int n = 0; n < R8; ++n) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
+    m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+  }
   __syncthreads();
 
   for (int at = 0; u < ue; u += kStride, at ^= 1) {
     cp_wait<1>();
     __syncwarp();
     const uint8_t *ks = ring.kv[at][0], *vs = ring.kv[at][1];
-    // S: two n-tiles of 8 keys per unit
-    float s[kPair][2][4] = {};
+    float s[kPair][R8][4];  // keys g (0, 1) and g + 8 (2, 3) of a unit, rows 2 c and 2 c + 1
+#pragma unroll
+    for (int p = 0; p < kPair; ++p)
+#pragma unroll
+      for (int n = 0; n < R8; ++n) s[p][n][0] = s[p][n][1] = s[p][n][2] = s[p][n][3] = 0.0f;
 #pragma unroll
     for (int r = 0; r < KR; ++r) {
       uint4 kc[kPair][2];
@@ -252,17 +276,20 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
         for (int t = 0; t < 2; ++t)
           kc[p][t] = *reinterpret_cast<const uint4*>(ks + chunk_at<DIM>(p * kUnit + t * 8 + g, r * 4 + c));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 q = sm.q[r * 4 + i][lane];
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int p = 0; p < kPair; ++p)
+        for (int p = 0; p < kPair; ++p) {
+          const uint4 &lo = kc[p][0], &hi = kc[p][1];
+          const uint32_t x = (i == 0 ? lo.x : i == 1 ? lo.y : i == 2 ? lo.z : lo.w) ^ 0x80808080u;
+          const uint32_t y = (i == 0 ? hi.x : i == 1 ? hi.y : i == 2 ? hi.z : hi.w) ^ 0x80808080u;
+          const uint32_t a0 = f16_from_u8(x, 0x4140), a2 = f16_from_u8(x, 0x4342);
+          const uint32_t a1 = f16_from_u8(y, 0x4140), a3 = f16_from_u8(y, 0x4342);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const uint4& k4 = kc[p][t];
-            const uint32_t x = (i == 0 ? k4.x : i == 1 ? k4.y : i == 2 ? k4.z : k4.w) ^ 0x80808080u;
-            mma_f16(s[p][t], q.x, q.y, q.z, q.w, f16_from_u8(x, 0x4140), f16_from_u8(x, 0x4342));
+          for (int n = 0; n < R8; ++n) {
+            const uint2 b = R8 > 1 ? sm.q[R8 > 1 ? r * 4 + i : 0][n][lane] : qf[r * 4 + i];
+            mma_f16(s[p][n], a0, a1, a2, a3, b.x, b.y);
           }
-      }
+        }
     }
     // scores in powers of two, masked where the step crosses an edge of what some row sees
     const int k0 = u * kUnit;
@@ -273,54 +300,65 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
       const PageEntry e = sm.pages[((min(u + p, ue - 1) * kUnit) >> lg) - pg0];
       rv[p] = e.rv;
       whole = whole && e.pid >= 0;
-      const float f0 = e.ks * q_unit[0], f1 = e.ks * q_unit[1], lv = e.pid >= 0 && u + p < ue ? e.lv : -INFINITY;
+      const float lv = e.pid >= 0 && u + p < ue ? e.lv : -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[p][t][0] = fmaf(s[p][t][0], f0, lv), s[p][t][1] = fmaf(s[p][t][1], f0, lv);
-        s[p][t][2] = fmaf(s[p][t][2], f1, lv), s[p][t][3] = fmaf(s[p][t][3], f1, lv);
-      }
+      for (int n = 0; n < R8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[p][n][i] = fmaf(s[p][n][i], e.ks * q_unit[n][i & 1], lv);
     }
     if (__builtin_expect(!whole, 0)) {
 #pragma unroll
       for (int p = 0; p < kPair; ++p)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int n = 0; n < R8; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = k0 + p * kUnit + 8 * t + 2 * c + (i & 1);
-            if (key < see_lo[i >> 1] || key >= see_hi[i >> 1]) s[p][t][i] = -INFINITY;
+            const int key = k0 + p * kUnit + g + 8 * (i >> 1);
+            if (key < see_lo[n][i & 1] || key >= see_hi[n][i & 1]) s[p][n][i] = -INFINITY;
           }
     }
-    float top0 = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-    for (int p = 0; p < kPair; ++p) {
-      top0 = fmaxf(top0, fmaxf(fmaxf(s[p][0][0], s[p][0][1]), fmaxf(s[p][1][0], s[p][1][1])));
-      top1 = fmaxf(top1, fmaxf(fmaxf(s[p][0][2], s[p][0][3]), fmaxf(s[p][1][2], s[p][1][3])));
-    }
     // a thread's own scores say whether an offset has to move; the rows' maxima are looked up only then
-    if (__builtin_expect(__any_sync(0xffffffffu, top0 > m[0] + kMost || top1 > m[1] + kMost), 0)) {
-      top0 = quad_max(top0), top1 = quad_max(top1);
-      const float n0 = top0 > m[0] + kMost ? top0 - kTop : m[0], n1 = top1 > m[1] + kMost ? top1 - kTop : m[1];
-      const float b0 = m[0] == n0 ? 1.0f : ex2(m[0] - n0), b1 = m[1] == n1 ? 1.0f : ex2(m[1] - n1);
-      m[0] = n0, m[1] = n1;
-      l[0] *= b0, l[1] *= b1;
+    bool over = false;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) o[i][0] *= b0, o[i][1] *= b0, o[i][2] *= b1, o[i][3] *= b1;
+    for (int n = 0; n < R8; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < kPair; ++p) top = fmaxf(top, fmaxf(s[p][n][i], s[p][n][2 + i]));
+        over = over || top > m[n][i] + kMost;
+      }
+    if (__builtin_expect(__any_sync(0xffffffffu, over), 0)) {
+#pragma unroll
+      for (int n = 0; n < R8; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int p = 0; p < kPair; ++p) top = fmaxf(top, fmaxf(s[p][n][i], s[p][n][2 + i]));
+          top = rows_max(top);
+          const float to = top > m[n][i] + kMost ? top - kTop : m[n][i];
+          const float b = m[n][i] == to ? 1.0f : ex2(m[n][i] - to);
+          m[n][i] = to;
+          l[n][i] *= b;
+#pragma unroll
+          for (int j = 0; j < MT; ++j) o[j][n][i] *= b, o[j][n][2 + i] *= b;
+        }
     }
-    // a row that has seen nothing yet has m = -inf and only -inf scores
-    const float m0 = m[0] == -INFINITY ? 0.0f : m[0], m1 = m[1] == -INFINITY ? 0.0f : m[1];
 #pragma unroll
     for (int p = 0; p < kPair; ++p) {
-      float w[2][4];
+      uint32_t b0[R8], b1[R8];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        w[t][0] = ex2(s[p][t][0] - m0), w[t][1] = ex2(s[p][t][1] - m0);
-        w[t][2] = ex2(s[p][t][2] - m1), w[t][3] = ex2(s[p][t][3] - m1);
+      for (int n = 0; n < R8; ++n) {
+        // a row that has seen nothing yet has m = -inf and only -inf scores
+        const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+        const float w0 = ex2(s[p][n][0] - m0), w1 = ex2(s[p][n][1] - m1);
+        const float w2 = ex2(s[p][n][2] - m0), w3 = ex2(s[p][n][3] - m1);
+        l[n][0] = fmaf(w0 + w2, rv[p], l[n][0]);
+        l[n][1] = fmaf(w1 + w3, rv[p], l[n][1]);
+        b0[n] = transpose8(pack_f16(w0, w1));
+        b1[n] = transpose8(pack_f16(w2, w3));
       }
-      l[0] = fmaf((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]), rv[p], l[0]);
-      l[1] = fmaf((w[0][2] + w[0][3]) + (w[1][2] + w[1][3]), rv[p], l[1]);
-      const uint32_t a0 = pack_f16(w[0][0], w[0][1]), a1 = pack_f16(w[0][2], w[0][3]);
-      const uint32_t a2 = pack_f16(w[1][0], w[1][1]), a3 = pack_f16(w[1][2], w[1][3]);
       uint32_t vr[4][VW];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -336,17 +374,19 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
           }
         }
       }
-      // O: n-tile j holds elements (lane / 4) * DIM / 8 + j of the head
+      // O^T: m-tile j holds elements (lane / 4) * DIM / 8 + 2 j and the next of the head
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
         const uint32_t x0 = vr[0][i] ^ 0x80808080u, x1 = vr[1][i] ^ 0x80808080u;
         const uint32_t x2 = vr[2][i] ^ 0x80808080u, x3 = vr[3][i] ^ 0x80808080u;
-        const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
-        const uint32_t s0 = __byte_perm(x2, x3, 0x5140), s1 = __byte_perm(x2, x3, 0x7362);
-        mma_f16(o[4 * i], a0, a1, a2, a3, f16_from_u8(p0, 0x4140), f16_from_u8(s0, 0x4140));
-        mma_f16(o[4 * i + 1], a0, a1, a2, a3, f16_from_u8(p0, 0x4342), f16_from_u8(s0, 0x4342));
-        mma_f16(o[4 * i + 2], a0, a1, a2, a3, f16_from_u8(p1, 0x4140), f16_from_u8(s1, 0x4140));
-        mma_f16(o[4 * i + 3], a0, a1, a2, a3, f16_from_u8(p1, 0x4342), f16_from_u8(s1, 0x4342));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t p0 = __byte_perm(x0, x1, h ? 0x7362 : 0x5140), p1 = __byte_perm(x2, x3, h ? 0x7362 : 0x5140);
+          const uint32_t a0 = f16_from_u8(p0, 0x4140), a1 = f16_from_u8(p0, 0x4342);
+          const uint32_t a2 = f16_from_u8(p1, 0x4140), a3 = f16_from_u8(p1, 0x4342);
+#pragma unroll
+          for (int n = 0; n < R8; ++n) mma_f16(o[2 * i + h][n], a0, a1, a2, a3, b0[n], b1[n]);
+        }
       }
     }
     __syncwarp();
@@ -356,35 +396,36 @@ __global__ void __launch_bounds__(kWarps * 32, DIM == 256 ? 2 : DIM == 128 ? 3 :
   cp_wait<0>();
 
   // ---- the four warps' parts joined (the outputs take the place of the codes)
-  l[0] = quad_sum(l[0]), l[1] = quad_sum(l[1]);
-  if (c == 0) {
-    sm.ml[warp][g] = make_float2(m[0], l[0]);
-    sm.ml[warp][g + 8] = make_float2(m[1], l[1]);
-  }
+#pragma unroll
+  for (int n = 0; n < R8; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[n][i] = rows_sum(l[n][i]);
+      if (g == 0) sm.ml[warp][8 * n + 2 * c + i] = make_float2(m[n][i], l[n][i]);
+    }
   __syncthreads();  // also: no warp reads codes any more
 #pragma unroll
-  for (int rr = 0; rr < 2; ++rr) {
-    const int r = g + 8 * rr;
-    float top = -INFINITY;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.ml[w][r].x);
-    const float b = m[rr] == top ? 1.0f : exp2f(m[rr] - top);
-    if (r < nr) {
-      // thread's columns 2c, 2c + 1 of n-tile j are elements (2c) * NT + j and (2c + 1) * NT + j
+  for (int n = 0; n < R8; ++n)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        sm.o[warp][r][2 * c * NT + j] = o[j][2 * rr] * b;
-        sm.o[warp][r][(2 * c + 1) * NT + j] = o[j][2 * rr + 1] * b;
+    for (int i = 0; i < 2; ++i) {
+      const int r = 8 * n + 2 * c + i;
+      float top = -INFINITY;
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.ml[w][r].x);
+      const float b = m[n][i] == top ? 1.0f : ex2(m[n][i] - top);
+      if (r < nr) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          *reinterpret_cast<float2*>(&sm.o[warp][r][g * (DIM / 8) + 2 * j]) = make_float2(o[j][n][i] * b, o[j][n][2 + i] * b);
+      }
+      if (warp == 0 && g == 0) {
+        float sum = 0.0f;
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 x = sm.ml[w][r];
+          sum += x.x == top ? x.y : x.y * ex2(x.x - top);
+        }
+        sm.row_ml[r][0] = top, sm.row_ml[r][1] = sum;
       }
     }
-    if (warp == 0 && c == 0) {
-      float sum = 0.0f;
-      for (int w = 0; w < kWarps; ++w) {
-        const float2 x = sm.ml[w][r];
-        sum += x.x == top ? x.y : x.y * exp2f(x.x - top);
-      }
-      sm.row_ml[r][0] = top, sm.row_ml[r][1] = sum;
-    }
-  }
   __syncthreads();
   T* out = static_cast<T*>(a.out);
   for (int i = threadIdx.x; i < nr * (DIM / 2); i += blockDim.x) {
@@ -470,21 +511,21 @@ unsigned* tickets_of(int device) {
   return buf[device];
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, int R8>
 bool stream_launch(Call& c, const AttnArgs& a) {
-  constexpr int kBase = (int)sizeof(StreamSmem<DIM>), kMost = kBase + kMaxPages * (int)sizeof(PageEntry);
+  constexpr int kBase = (int)sizeof(StreamSmem<DIM, R8>), kMost = kBase + kMaxPages * (int)sizeof(PageEntry);
   static int per_sm[64] = {};  // blocks per SM with few pages, which is the case where it counts
   const int dv = current_device() & 63;
   if (!per_sm[dv]) {
     int n = 0;
-    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_stream<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost)) ||
-        !ACF_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn_stream<T, DIM>, kWarps * 32, kBase + 1024)))
+    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_attn_stream<T, DIM, R8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost)) ||
+        !ACF_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn_stream<T, DIM, R8>, kWarps * 32, kBase + 1024)))
       return false;
     per_sm[dv] = std::max(1, n);
   }
   StreamArgs p = {};
   p.a = a;
-  const long long tiles = ((long long)std::min(a.b.max_new, a.b.tokens) * a.group + 15) / 16;
+  const long long tiles = ((long long)std::min(a.b.max_new, a.b.tokens) * a.group + 8 * R8 - 1) / (8 * R8);
   if (tiles * a.kv.heads > 0x7fffffffLL) {
     set_error(kInvalid, "acfun_kv8_attention: too many rows");
     return false;
@@ -520,8 +561,18 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     if (!c.ok() || !p.tickets) return false;
   }
   const int smem = kBase + (int)std::min<long long>(chunk / a.kv.page + 2, kMaxPages) * (int)sizeof(PageEntry);
-  k_attn_stream<T, DIM><<<dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), kWarps * 32, smem, c.stream()>>>(p, c.err());
+  k_attn_stream<T, DIM, R8><<<dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), kWarps * 32, smem, c.stream()>>>(p, c.err());
   return c.launched("k_attn_stream");
+}
+
+template <typename T, int DIM>
+bool stream_rows(Call& c, const AttnArgs& a) {
+  // the widest tile that the rows fill: each tile reads (from L2, after the first) and converts the
+  // keys again.  32 rows of 256 elements do not fit in the registers.
+  const long long rows = (long long)std::min(a.b.max_new, a.b.tokens) * a.group;
+  if (rows <= 8) return stream_launch<T, DIM, 1>(c, a);
+  if (rows <= 16 || DIM == 256) return stream_launch<T, DIM, 2>(c, a);
+  return stream_launch<T, DIM, DIM == 256 ? 2 : 4>(c, a);
 }
 
 }  // namespace
@@ -529,10 +580,10 @@ bool stream_launch(Call& c, const AttnArgs& a) {
 bool attn_stream_dev(Call& c, const AttnArgs& a) {
   const int d = a.kv.dim;
   if (a.dtype == ACFUN_F16)
-    return d == 64 ? stream_launch<__half, 64>(c, a) : d == 128 ? stream_launch<__half, 128>(c, a)
-                                                                 : stream_launch<__half, 256>(c, a);
-  return d == 64 ? stream_launch<__nv_bfloat16, 64>(c, a) : d == 128 ? stream_launch<__nv_bfloat16, 128>(c, a)
-                                                                      : stream_launch<__nv_bfloat16, 256>(c, a);
+    return d == 64 ? stream_rows<__half, 64>(c, a) : d == 128 ? stream_rows<__half, 128>(c, a) : stream_rows<__half, 256>(c, a);
+  return d == 64    ? stream_rows<__nv_bfloat16, 64>(c, a)
+         : d == 128 ? stream_rows<__nv_bfloat16, 128>(c, a)
+                    : stream_rows<__nv_bfloat16, 256>(c, a);
 }
 
 }  // namespace acf
