@@ -204,29 +204,32 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
   float q_unit[R8][2];  // of rows 2 c, 2 c + 1 of each eight
   {
     const T* q = static_cast<const T*>(a.q);
+    const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && a.q_token % 8 == 0 && a.q_head % 8 == 0;
 #pragma unroll
     for (int n = 0; n < R8; ++n) {
       const int r = r0 + 8 * n + g;
       const bool in = 8 * n + g < nr;
       const int t = r / a.group, hq = head * a.group + r - t * a.group;
       const T* src = q + (long long)(sv.row0 + t) * a.q_token + (long long)hq * a.q_head + c * 16;
-      float top = 0.0f;
-      if (in) {
+      float x[KR][2][8], top = 0.0f;  // 16 elements of each run of 64
 #pragma unroll
-        for (int i = 0; i < DIM / 16; ++i)
+      for (int i = 0; i < KR; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to_f(src[(i / 4) * 64 + 4 * (i % 4) + e])));
-      }
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[i][h][e] = 0.0f;
+          if (in) load8(src + i * 64 + 8 * h, vec, x[i][h]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][h][e]));
+        }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const Pow2 w = row_pow2(top);
 #pragma unroll
       for (int i = 0; i < DIM / 16; ++i) {
         if (R8 > 1 && i % kWarps != warp) continue;
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = in ? to_f(src[(i / 4) * 64 + 4 * (i % 4) + e]) * w.down : 0.0f;
-        qf[i] = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
+        const float* y = &x[i / 4][(i % 4) >> 1][4 * (i & 1)];
+        qf[i] = make_uint2(pack_f16(y[0] * w.down, y[1] * w.down), pack_f16(y[2] * w.down, y[3] * w.down));
         if constexpr (R8 > 1) sm.q[i][n][lane] = qf[i];
       }
       q_unit[n][0] = __shfl_sync(0xffffffffu, w.up, 8 * c);
@@ -531,13 +534,16 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     return false;
   }
   p.row_tiles = (int)tiles;
-  // Split the keys so that one wave of resident blocks covers the batch; sequences of a batch may
-  // differ in length, and chunks of at most 1024 keys keep its longest from being the last.
+  // Split the keys so that one wave of resident blocks covers the batch.  Sequences of a batch may
+  // differ in length: chunks of about 1024 keys keep the longest from being the last (48 ragged
+  // sequences: 512 keys 73 us, 1024 and 2048 59 us), longer ones only where these would make more
+  // than 16 waves of blocks.  Blocks that walk a list of the chunks there are, made from the lengths
+  // in the kernel, took 61 us: their start has to wait for the list.
   const long long work = tiles * a.kv.heads * a.b.seqs;
   const long long slots = (long long)per_sm[dv] * c.sm_count();
   const long long want = std::max<long long>(1, slots / std::max<long long>(1, work));
   long long chunk = (a.b.max_len + want - 1) / want;
-  if (a.b.seqs > 1) chunk = std::min<long long>(chunk, 1024);
+  if (a.b.seqs > 1) chunk = std::min(chunk, std::max<long long>(1024, work * a.b.max_len / (16 * slots)));
   chunk = std::max<long long>(chunk, kUnit * kPair * kWarps);
   chunk = std::min<long long>((chunk + kUnit - 1) / kUnit * kUnit, (long long)(kMaxPages - 1) * a.kv.page);
   p.chunk = (int)chunk;
