@@ -136,6 +136,8 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
   extern __shared__ __align__(128) uint8_t smem_raw[];
   using Smem = StreamSmem<DIM, R8>;
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
   const AttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int head = blockIdx.x % a.kv.heads, rt = blockIdx.x / a.kv.heads, seq = blockIdx.y, chunk_i = blockIdx.z;
@@ -567,7 +569,8 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     if (!c.ok() || !p.tickets) return false;
   }
   const int smem = kBase + (int)std::min<long long>(chunk / a.kv.page + 2, kMaxPages) * (int)sizeof(PageEntry);
-  k_attn_stream<T, DIM, R8><<<dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), kWarps * 32, smem, c.stream()>>>(p, c.err());
+  if (!ACF_CUDA_OK(launch_pdl(k_attn_stream<T, DIM, R8>, dim3(p.row_tiles * a.kv.heads, a.b.seqs, p.splits), dim3(kWarps * 32), (size_t)smem, c.stream(), p, c.err())))
+    return false;
   return c.launched("k_attn_stream");
 }
 

@@ -145,6 +145,8 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   extern __shared__ float2 cs[];  // [tokens in this page][rot / 2], keys only
   __shared__ float warp_max[2][32];
   constexpr int UPR = DIM / 16;  // units per row
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
   const int seq = blockIdx.z, page = a.kv.page;
   const bool is_v = blockIdx.y & 1;
   const SeqView sv = seq_view(a.b, seq, err);
@@ -306,7 +308,9 @@ bool append_launch(Call& c, AppendArgs a) {
       return false;
     attr_done[dv & 63] = true;
   }
-  k_kv8_append<T, DIM><<<dim3(slots, 2 * parts, a.b.seqs), threads, smem, c.stream()>>>(a, c.err());
+  if (!ACF_CUDA_OK(launch_pdl(k_kv8_append<T, DIM>, dim3(slots, 2 * parts, a.b.seqs), dim3(threads), smem, c.stream(), a,
+                              c.err())))
+    return false;
   return c.launched("k_kv8_append");
 }
 
@@ -323,6 +327,8 @@ struct ReadArgs {
 // of it.  Codes of neighbouring heads are contiguous; a thread turns 16 codes into values.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256) k_kv8_read(const ReadArgs a, unsigned* err) {
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
   const int seq = blockIdx.z, page = a.kv.page;
   const SeqView sv = seq_view(a.b, seq, err);
   const int first = sv.len - sv.n;
@@ -376,7 +382,8 @@ bool read_launch(Call& c, ReadArgs a) {
   // a block takes the heads that make about two passes of its 256 threads
   a.head_block = std::max(1, std::min(a.kv.heads, 512 * 16 / (page * DIM)));
   const int parts = (a.kv.heads + a.head_block - 1) / a.head_block;
-  k_kv8_read<T, DIM><<<dim3(slots, parts, a.b.seqs), 256, 0, c.stream()>>>(a, c.err());
+  if (!ACF_CUDA_OK(launch_pdl(k_kv8_read<T, DIM>, dim3(slots, parts, a.b.seqs), dim3(256), 0, c.stream(), a, c.err())))
+    return false;
   return c.launched("k_kv8_read");
 }
 

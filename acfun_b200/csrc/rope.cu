@@ -31,6 +31,8 @@ struct RopeArgs {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_rope(const RopeArgs a) {
   extern __shared__ float2 cs[];  // [tok_block][rot / 2]
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
   const int half = a.rot / 2;
   const int t0 = blockIdx.x * a.tok_block, nt = min(a.tok_block, a.tokens - t0);
   const int h0 = blockIdx.y * a.head_block, nh = min(a.head_block, a.heads - h0);
@@ -129,10 +131,8 @@ bool rope_launch(Call& c, RopeArgs a) {
     return false;
   }
   const size_t smem = (size_t)a.tok_block * (a.rot / 2) * sizeof(float2);
-  if (vec)
-    k_rope<T, true><<<dim3(blocks, parts), 256, smem, c.stream()>>>(a);
-  else
-    k_rope<T, false><<<dim3(blocks, parts), 256, smem, c.stream()>>>(a);
+  if (!ACF_CUDA_OK(launch_pdl(vec ? k_rope<T, true> : k_rope<T, false>, dim3(blocks, parts), dim3(256), smem, c.stream(), a)))
+    return false;
   return c.launched("k_rope");
 }
 

@@ -12,17 +12,22 @@ import numpy as np
 
 from . import AcfunError, check, lib
 
-_DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
-_codes = {}
+_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int32": 10, "int8": 11}
+_F32, _I32, _I8 = 0, 10, 11
+_codes = {}  # by dtype object: these calls cost a few microseconds, and naming a dtype is one of them
+
+
+def _code(dt):
+    code = _codes.get(dt)
+    if code is None:
+        code = _codes[dt] = _TYPES.get(str(dt).replace("torch.", ""), -1)
+    return code
 
 
 def _dtype_code(dt):
-    code = _codes.get(dt)
-    if code is None:
-        code = _DTYPES.get(str(dt).replace("torch.", ""))
-        if code is None:
-            raise TypeError(f"dtype {dt} is not float32, float16 or bfloat16")
-        _codes[dt] = code
+    code = _code(dt)
+    if not 0 <= code <= 2:
+        raise TypeError(f"dtype {dt} is not float32, float16 or bfloat16")
     return code
 
 
@@ -44,14 +49,10 @@ def _address(x):
     return x.ctypes.data if isinstance(x, np.ndarray) else x.data_ptr()
 
 
-def _flat(x, dtype, what):
+def _flat(x, code, what):
     """The address of a contiguous array of the given element type."""
-    if isinstance(x, np.ndarray):
-        ok = x.flags["C_CONTIGUOUS"] and x.dtype.name == dtype
-    else:
-        ok = x.is_contiguous() and str(x.dtype) == "torch." + dtype
-    if not ok:
-        raise ValueError(f"{what} must be contiguous {dtype}")
+    if not (x.flags["C_CONTIGUOUS"] if isinstance(x, np.ndarray) else x.is_contiguous()) or _code(x.dtype) != code:
+        raise ValueError(f"{what} must be contiguous {[k for k, v in _TYPES.items() if v == code][0]}")
     return _address(x)
 
 
@@ -68,11 +69,12 @@ def _strides(x, what):
     return t, h
 
 
-def _empty(like, shape, dtype=None):
-    if isinstance(like, np.ndarray):
-        return np.empty(shape, dtype=dtype or like.dtype)
+def _like(x):
+    """An uninitialised array of x's shape and dtype, where x is."""
+    if isinstance(x, np.ndarray):
+        return np.empty(x.shape, x.dtype)
     import torch
-    return torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
+    return torch.empty_like(x)
 
 
 def _done(code):
@@ -89,7 +91,7 @@ class Rope:
         if freq.ndim != 1:
             raise ValueError("freq must have one dimension")
         self.freq = freq
-        self.c = _Rope(_flat(freq, "float32", "freq"), 2 * freq.shape[0], int(bool(interleaved)), float(amplitude))
+        self.c = _Rope(_flat(freq, _F32, "freq"), 2 * freq.shape[0], int(bool(interleaved)), float(amplitude))
         self.ref = C.byref(self.c)
 
 
@@ -114,15 +116,16 @@ def rope_frequencies(rot, base=10000.0, scaling=None, factor=1.0, trained=0, fas
 def rope(x, positions, spec: Rope, out=None):
     """x [tokens, heads, dim] at int32 positions [tokens]; out may be x."""
     t, h = _strides(x, "x")
-    if positions.shape != (x.shape[0],):
+    tokens, heads, dim = x.shape
+    if positions.shape != (tokens,):
         raise ValueError("positions must be [tokens]")
     if out is None:
-        out = _empty(x, x.shape)
+        out = _like(x)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must have x's shape and dtype")
     ot, oh = _strides(out, "out")
-    _done(lib().acfun_rope(_address(x), _address(out), _dtype_code(x.dtype), x.shape[0], x.shape[1], x.shape[2], t, h,
-                           ot, oh, _flat(positions, "int32", "positions"), spec.ref))
+    _done(lib().acfun_rope(_address(x), _address(out), _dtype_code(x.dtype), tokens, heads, dim, t, h, ot, oh,
+                           _flat(positions, _I32, "positions"), spec.ref))
     return out
 
 
@@ -138,8 +141,8 @@ class KvBatch:
             raise ValueError("table must be [seqs, columns], start [seqs + 1] and length [seqs]")
         self.arrays = (table, start, length)
         self.tokens = int(tokens)
-        self.c = _Batch(_flat(table, "int32", "table"), _flat(start, "int32", "start"),
-                        _flat(length, "int32", "length"), table.shape[0], table.shape[1], self.tokens, int(max_new),
+        self.c = _Batch(_flat(table, _I32, "table"), _flat(start, _I32, "start"),
+                        _flat(length, _I32, "length"), table.shape[0], table.shape[1], self.tokens, int(max_new),
                         int(max_len))
         self.ref = C.byref(self.c)
 
@@ -153,8 +156,8 @@ class KvCache8:
             raise ValueError("codes must be [pages, heads, page, dim], scales [pages, heads]")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page, self.dim = k.shape
-        self.c = _Cache(_flat(k, "int8", "k"), _flat(v, "int8", "v"), _flat(k_scale, "float32", "k_scale"),
-                        _flat(v_scale, "float32", "v_scale"), *k.shape)
+        self.c = _Cache(_flat(k, _I8, "k"), _flat(v, _I8, "v"), _flat(k_scale, _F32, "k_scale"),
+                        _flat(v_scale, _F32, "v_scale"), *k.shape)
         self.ref = C.byref(self.c)
 
     @classmethod
@@ -182,8 +185,7 @@ class KvCache8:
 
     def read(self, batch: KvBatch, dtype):
         """(k, v) [tokens, heads, dim]: the last start[i + 1] - start[i] tokens of each sequence."""
-        shape = (batch.tokens, self.heads, self.dim)
-        k, v = _empty(self.k, shape, dtype), _empty(self.k, shape, dtype)
+        k, v = self.k.new_empty((2, batch.tokens, self.heads, self.dim), dtype=dtype).unbind()
         _done(lib().acfun_kv8_read(self.ref, batch.ref, k.data_ptr(), v.data_ptr(), _dtype_code(dtype)))
         return k, v
 
@@ -194,7 +196,7 @@ class KvCache8:
         if q.shape[0] != batch.tokens or q.shape[2] != self.dim:
             raise ValueError(f"q must be [{batch.tokens}, q_heads, {self.dim}], got {tuple(q.shape)}")
         if out is None:
-            out = _empty(q, q.shape)
+            out = _like(q)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out must have q's shape and dtype")
         if lse is not None and tuple(lse.shape) != tuple(q.shape[:2]):
@@ -203,5 +205,5 @@ class KvCache8:
         _done(lib().acfun_kv8_attention(self.ref, batch.ref, _address(q), _address(out), _dtype_code(q.dtype),
                                         q.shape[1], qt, qh, ot, oh, self.dim ** -0.5 if scale is None else scale,
                                         int(bool(causal)), window,
-                                        _flat(lse, "float32", "lse") if lse is not None else None))
+                                        _flat(lse, _F32, "lse") if lse is not None else None))
         return out
