@@ -95,6 +95,24 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = to_f(p[i]);
   }
 }
+// The same in two steps, so that a load can be under way while other work is done.
+template <typename T>
+struct Raw8 {
+  union {
+    uint4 u[sizeof(T) / 2];
+    T t[8];
+  };
+};
+template <typename T>
+__device__ __forceinline__ void load8_raw(const T* p, bool vec, Raw8<T>& r) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.t[i] = p[i];
+  }
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
   if (vec) {

@@ -117,34 +117,38 @@ struct AppendArgs {
   int head_block;  // heads of one block
 };
 
-__device__ __forceinline__ float quant_fixup(float x) {
-  // NaN counts as 0, infinities as the largest finite value when coded
-  return x != x ? 0.0f : x;
+// The larger of a and |b|; NaN when either is.
+__device__ __forceinline__ float amax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+  return d;
 }
-__device__ __forceinline__ uint32_t code_of(float x, float unit) {
-  float r = rintf(__fmul_rn(x, unit));
-  r = fminf(fmaxf(r, -127.0f), 127.0f);
-  return (uint32_t)(int)r & 0xffu;
-}
+constexpr float kFinite = 3.4028234663852886e38f;
+
+// rint(x * unit) of eight values, |x * unit| < 127.5, as bytes: adding 1.5 * 2^23 rounds to an integer
+// (ties to even, as rint) that stands in the sum's low byte.
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float unit) {
-  uint2 w = make_uint2(0, 0);
+  uint32_t b[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w.x |= code_of(x[i], unit) << (8 * i);
-    w.y |= code_of(x[4 + i], unit) << (8 * i);
-  }
-  return w;
+  for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], unit), 12582912.0f));
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
+template <int DIM>
+constexpr int kUnits = DIM == 256 ? 2 : 1;
+
 // One block: page slot blockIdx.x of the new tokens of sequence blockIdx.z, heads
-// [blockIdx.y / 2 * head_block, ...), keys (blockIdx.y even) or values (odd).  A thread holds two
-// units of 16 elements of the tile in registers between the maximum and the coding: two runs of 8
-// elements, which in the half layout are the two sides of 8 pairs.  page * DIM / 32 threads.
+// [blockIdx.y / 2 * head_block, ...), keys (blockIdx.y even) or values (odd).  A head takes page * DIM
+// / 16 threads, so that small pages have several heads in a block at a time.  A thread holds a
+// unit of 16 elements of the tile (two of them when dim is 256) in registers between the maximum and
+// the coding: two runs of 8 elements, which in the half layout are the two sides of 8 pairs.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigned* err) {
-  extern __shared__ float2 cs[];  // [tokens in this page][rot / 2], keys only
-  __shared__ float warp_max[2][32];
+  extern __shared__ __align__(16) float2 cs[];  // [tokens in this page][rot / 2], keys only
+  __shared__ float warp_max[2][2][32];
   constexpr int UPR = DIM / 16;  // units per row
+  constexpr int UN = kUnits<DIM>;
   dev::grid_dep_wait();
   dev::grid_dep_launch();
   const int seq = blockIdx.z, page = a.kv.page;
@@ -166,17 +170,29 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   const int half = a.rot / 2;
   const bool turn = !is_v && a.rot > 0;
   if (turn) {
-    for (int i = threadIdx.x; i < (hi - lo) * half; i += blockDim.x) {
-      const int t = i / half;
-      cs[i] = rope_cs(g * page + lo + t, a.freq[i - t * half], a.amp);
+    // A thread takes a pair's run of consecutive tokens: the first angle is computed, the others
+    // are turned on from it by one position's angle (at most 127 turns, each within 2^-23).
+    const int n = hi - lo, runs = max(1, (int)blockDim.x / half), len = (n + runs - 1) / runs;
+    for (int i = threadIdx.x; i < half * runs; i += blockDim.x) {
+      const int t0 = i / half * len, pair = i % half;
+      if (t0 >= n) continue;
+      const float f = a.freq[pair];
+      float2 w = rope_cs(g * page + lo + t0, f, a.amp);
+      const float2 one = len > 1 ? rope_cs(1, f, 1.0f) : make_float2(1.0f, 0.0f);
+      for (int t = t0; t < min(t0 + len, n); ++t) {
+        cs[t * half + pair] = w;
+        w = make_float2(w.x * one.x - w.y * one.y, w.y * one.x + w.x * one.y);
+      }
     }
     __syncthreads();
   }
+  const int per_head = page * DIM / (16 * UN), group = threadIdx.x / per_head, groups = blockDim.x / per_head;
+  const int tid = threadIdx.x - group * per_head;
   // this thread's units: slot and the element offsets of their two runs
-  int slot[2], at0[2], at1[2], cs_at[2];
+  int slot[UN], at0[UN], at1[UN], cs_at[UN];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int idx = threadIdx.x + j * blockDim.x;
+  for (int j = 0; j < UN; ++j) {
+    const int idx = tid + j * per_head;
     const int u = idx % UPR;
     slot[j] = idx / UPR;
     cs_at[j] = -1;
@@ -199,88 +215,138 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   int8_t* codes = is_v ? a.kv.v : a.kv.k;
   float* scales = is_v ? a.kv.vs : a.kv.ks;
 
-  for (int h = h0; h < h1; ++h) {
-    float x[2][2][8];
-    float top = 127.0f * 0x1p-60f;
+  const int w0 = group * per_head / 32, w1 = w0 + per_head / 32;  // the head's warps
+  Raw8<T> raw[UN][2];
+  auto request = [&](int h) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (slot[j] >= lo && slot[j] < hi) {
+    for (int j = 0; j < UN; ++j) {
+      if (h < h1 && slot[j] >= lo && slot[j] < hi) {
         const T* p = src + (long long)(row_of_slot0 + slot[j]) * tok_stride + h * head_stride;
-        load8(p + at0[j], vec, x[j][0]);
-        load8(p + at1[j], vec, x[j][1]);
+        load8_raw(p + at0[j], vec, raw[j][0]);
+        load8_raw(p + at1[j], vec, raw[j][1]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][0][i] = x[j][1][i] = 0.0f;
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[j][0].u[i] = raw[j][1].u[i] = make_uint4(0, 0, 0, 0);
       }
     }
+  };
+  request(h0 + group);
+  for (int hb = h0, buf = 0; hb < h1; hb += groups, buf ^= 1) {
+    const int h = min(hb + group, h1 - 1);
+    const bool mine = hb + group < h1;  // a group without a head of its own only keeps the barriers
+    float x[UN][2][8];
+    float top = 127.0f * 0x1p-60f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < UN; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[j][r][i] = to_f(raw[j][r].t[i]);
+    request(hb + groups + group);  // the next head's values, while this one's are worked on
+    const size_t sc = (size_t)pid * a.kv.heads + h;
+    const float before = lo > 0 ? scales[sc] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < UN; ++j) {
       if (slot[j] >= lo && slot[j] < hi && cs_at[j] >= 0) {
-        const float2* w = cs + cs_at[j];
+        const float4* w = reinterpret_cast<const float4*>(cs + cs_at[j]);  // 8 pairs from a multiple of 8
         if (a.interleaved) {
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 c = w[4 * r + i];
-              const float p = x[j][r][2 * i], q = x[j][r][2 * i + 1];
-              x[j][r][2 * i] = p * c.x - q * c.y;
-              x[j][r][2 * i + 1] = q * c.x + p * c.y;
+            for (int i = 0; i < 4; i += 2) {
+              const float4 c = w[(4 * r + i) / 2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float cc = k ? c.z : c.x, ss = k ? c.w : c.y;
+                const float p = x[j][r][2 * (i + k)], q = x[j][r][2 * (i + k) + 1];
+                x[j][r][2 * (i + k)] = p * cc - q * ss;
+                x[j][r][2 * (i + k) + 1] = q * cc + p * ss;
+              }
             }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 c = w[i];
-            const float p = x[j][0][i], q = x[j][1][i];
-            x[j][0][i] = p * c.x - q * c.y;
-            x[j][1][i] = q * c.x + p * c.y;
+          for (int i = 0; i < 8; i += 2) {
+            const float4 c = w[i / 2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float cc = k ? c.z : c.x, ss = k ? c.w : c.y;
+              const float p = x[j][0][i + k], q = x[j][1][i + k];
+              x[j][0][i + k] = p * cc - q * ss;
+              x[j][1][i + k] = q * cc + p * ss;
+            }
           }
         }
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[j][r][i] = quant_fixup(x[j][r][i]);
-          const float m = fabsf(x[j][r][i]);
-          if (m <= 3.4028234663852886e38f) top = fmaxf(top, m);
-        }
+        for (int i = 0; i < 8; ++i) top = amax_nan(top, x[j][r][i]);
     }
-    // block maximum; the buffers alternate so that one barrier per head is enough
-    float* wm = warp_max[h & 1];
+    // the head's maximum; the buffers alternate so that one barrier per round is enough
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = amax_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) warp_max[0][buf][threadIdx.x >> 5] = top;
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    const float m = lane < (int)blockDim.x / 32 ? warp_max[0][buf][lane] : 0.0f;  // at most 32 warps
+    const bool finite = __all_sync(0xffffffffu, m <= kFinite);
+    top = lane >= w0 && lane < w1 ? m : 0.0f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0) wm[threadIdx.x >> 5] = top;
-    const size_t sc = (size_t)pid * a.kv.heads + h;
-    const float before = lo > 0 ? scales[sc] : 0.0f;
-    __syncthreads();
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) top = fmaxf(top, wm[w]);
+    if (__builtin_expect(!finite, 0)) {  // somewhere in the block: all look for their finite maximum
+      top = 127.0f * 0x1p-60f;
+#pragma unroll
+      for (int j = 0; j < UN; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (x[j][r][i] != x[j][r][i]) x[j][r][i] = 0.0f;
+            if (fabsf(x[j][r][i]) <= kFinite) top = fmaxf(top, fabsf(x[j][r][i]));
+          }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if ((threadIdx.x & 31) == 0) warp_max[1][buf][threadIdx.x >> 5] = top;
+      __syncthreads();
+      for (int w = w0; w < w1; ++w) top = fmaxf(top, warp_max[1][buf][w]);
+    }
     const float scale = fmaxf(before, __fdiv_rn(top, 127.0f));
     const float unit = __frcp_rn(scale);
-    int8_t* tile = codes + sc * page * DIM;
-    if (scale > before && lo > 0) {  // older tokens of the page move to the larger scale
-      const float f = __fdiv_rn(before, scale);
-      for (int i = threadIdx.x; i < lo * (DIM / 4); i += blockDim.x) {
-        uint32_t w = reinterpret_cast<uint32_t*>(tile)[i], r = 0;
+    if (__builtin_expect(!finite, 0)) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) r |= code_of((float)(int8_t)(w >> (8 * b)), f) << (8 * b);
-        reinterpret_cast<uint32_t*>(tile)[i] = r;
+      for (int j = 0; j < UN; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (fabsf(x[j][r][i]) > kFinite) x[j][r][i] = copysignf(scale * 127.0f, x[j][r][i]);
+    }
+    int8_t* tile = codes + sc * page * DIM;
+    if (mine && scale > before && lo > 0) {  // older tokens of the page move to the larger scale
+      const float f = __fdiv_rn(before, scale);
+      for (int i = tid; i < lo * (DIM / 8); i += per_head) {
+        uint2* at = reinterpret_cast<uint2*>(tile) + i;
+        const uint2 w = *at;
+        float y[8];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) y[b] = (float)(int8_t)(w.x >> (8 * b)), y[4 + b] = (float)(int8_t)(w.y >> (8 * b));
+        *at = codes8(y, f);
       }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (slot[j] < lo || slot[j] >= hi) continue;
+    for (int j = 0; j < UN; ++j) {
+      if (!mine || slot[j] < lo || slot[j] >= hi) continue;
       int8_t* o = tile + slot[j] * DIM;
-      const uint2 w0 = codes8(x[j][0], unit), w1 = codes8(x[j][1], unit);
+      const uint2 c0 = codes8(x[j][0], unit), c1 = codes8(x[j][1], unit);
       if (at1[j] == at0[j] + 8) {
-        *reinterpret_cast<uint4*>(o + at0[j]) = make_uint4(w0.x, w0.y, w1.x, w1.y);
+        *reinterpret_cast<uint4*>(o + at0[j]) = make_uint4(c0.x, c0.y, c1.x, c1.y);
       } else {
-        *reinterpret_cast<uint2*>(o + at0[j]) = w0;
-        *reinterpret_cast<uint2*>(o + at1[j]) = w1;
+        *reinterpret_cast<uint2*>(o + at0[j]) = c0;
+        *reinterpret_cast<uint2*>(o + at1[j]) = c1;
       }
     }
     // every thread has read the old scale before the barrier above
-    if (threadIdx.x == 0) scales[sc] = scale;
+    if (mine && tid == 0) scales[sc] = scale;
   }
   // new tokens past the last page slot of the grid
   if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1 && (g + 1) * (long long)page < sv.len)
@@ -290,7 +356,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
 template <typename T, int DIM>
 bool append_launch(Call& c, AppendArgs a) {
   const int page = a.kv.page;
-  const int threads = page * DIM / 32;
+  const int per_head = page * DIM / (16 * kUnits<DIM>);
   // pages that a run of max_new tokens can touch
   const int slots = std::max(1, (std::min(a.b.max_new, a.b.max_len) + page - 2) / page + 1);
   // All heads of a page in one block share its cosines and sines; with few pages the heads go to
@@ -299,6 +365,7 @@ bool append_launch(Call& c, AppendArgs a) {
   int parts = (int)std::min<long long>(a.kv.heads, std::max<long long>(1, 4LL * c.sm_count() / std::max<long long>(1, pages)));
   a.head_block = (a.kv.heads + parts - 1) / parts;
   parts = (a.kv.heads + a.head_block - 1) / a.head_block;
+  const int threads = per_head * std::max(1, std::min(a.head_block, 256 / per_head));
   const size_t smem = (size_t)std::min(page, a.b.max_new) * (a.rot / 2) * sizeof(float2);
   static bool attr_done[64] = {false};
   const int dv = current_device();
@@ -315,6 +382,11 @@ bool append_launch(Call& c, AppendArgs a) {
 }
 
 // ------------------------------------------------------------------ read
+// Byte i of a word of codes, each XORed with 0x80, as a float: under the exponent of 2^23 it is
+// 2^23 + code + 128, and the difference is exact.
+__device__ __forceinline__ float code_value(uint32_t w, int i) {
+  return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 | i)) - 8388736.0f;
+}
 struct ReadArgs {
   KvView kv;
   BatchView b;
@@ -368,7 +440,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const ReadArgs a, unsigned* er
       for (int e = 0; e < 2; ++e) {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)(words[2 * e + j / 4] >> (8 * (j % 4))) * s;
+        for (int j = 0; j < 8; ++j) x[j] = code_value(words[2 * e + j / 4] ^ 0x80808080u, j % 4) * s;
         store8(o + to + 8 * e, true, x);
       }
     }
