@@ -123,6 +123,12 @@ __device__ __forceinline__ float amax_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
   return d;
 }
+// The same over a warp.
+__device__ __forceinline__ float warp_max_nan(float a) {
+  float d;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
+  return d;
+}
 constexpr float kFinite = 3.4028234663852886e38f;
 
 // rint(x * unit) of eight values, |x * unit| < 127.5, as bytes: adding 1.5 * 2^23 rounds to an integer
@@ -217,22 +223,31 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
 
   const int w0 = group * per_head / 32, w1 = w0 + per_head / 32;  // the head's warps
   Raw8<T> raw[UN][2];
+  bool in[UN];
+  const T* from[UN];  // of the next head to request
+  int8_t* to[UN];     // of the head at hand
+  size_t sc = (size_t)pid * a.kv.heads + h0 + group;
+#pragma unroll
+  for (int j = 0; j < UN; ++j) {
+    in[j] = slot[j] >= lo && slot[j] < hi;
+    from[j] = src + (long long)(row_of_slot0 + slot[j]) * tok_stride + (h0 + group) * head_stride;
+    to[j] = codes + sc * page * DIM + slot[j] * DIM;
+  }
   auto request = [&](int h) {
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
-      if (h < h1 && slot[j] >= lo && slot[j] < hi) {
-        const T* p = src + (long long)(row_of_slot0 + slot[j]) * tok_stride + h * head_stride;
-        load8_raw(p + at0[j], vec, raw[j][0]);
-        load8_raw(p + at1[j], vec, raw[j][1]);
+      if (h < h1 && in[j]) {
+        load8_raw(from[j] + at0[j], vec, raw[j][0]);
+        load8_raw(from[j] + at1[j], vec, raw[j][1]);
       } else {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[j][0].u[i] = raw[j][1].u[i] = make_uint4(0, 0, 0, 0);
       }
+      from[j] += groups * head_stride;
     }
   };
   request(h0 + group);
   for (int hb = h0, buf = 0; hb < h1; hb += groups, buf ^= 1) {
-    const int h = min(hb + group, h1 - 1);
     const bool mine = hb + group < h1;  // a group without a head of its own only keeps the barriers
     float x[UN][2][8];
     float top = 127.0f * 0x1p-60f;
@@ -243,11 +258,10 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[j][r][i] = to_f(raw[j][r].t[i]);
     request(hb + groups + group);  // the next head's values, while this one's are worked on
-    const size_t sc = (size_t)pid * a.kv.heads + h;
-    const float before = lo > 0 ? scales[sc] : 0.0f;
+    const float before = lo > 0 && mine ? scales[sc] : 0.0f;
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
-      if (slot[j] >= lo && slot[j] < hi && cs_at[j] >= 0) {
+      if (in[j] && cs_at[j] >= 0) {
         const float4* w = reinterpret_cast<const float4*>(cs + cs_at[j]);  // 8 pairs from a multiple of 8
         if (a.interleaved) {
 #pragma unroll
@@ -283,16 +297,13 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
         for (int i = 0; i < 8; ++i) top = amax_nan(top, x[j][r][i]);
     }
     // the head's maximum; the buffers alternate so that one barrier per round is enough
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = amax_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = warp_max_nan(top);
     if ((threadIdx.x & 31) == 0) warp_max[0][buf][threadIdx.x >> 5] = top;
     __syncthreads();
     const int lane = threadIdx.x & 31;
     const float m = lane < (int)blockDim.x / 32 ? warp_max[0][buf][lane] : 0.0f;  // at most 32 warps
     const bool finite = __all_sync(0xffffffffu, m <= kFinite);
-    top = lane >= w0 && lane < w1 ? m : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = warp_max_nan(lane >= w0 && lane < w1 ? m : 0.0f);
     if (__builtin_expect(!finite, 0)) {  // somewhere in the block: all look for their finite maximum
       top = 127.0f * 0x1p-60f;
 #pragma unroll
@@ -321,11 +332,10 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
           for (int i = 0; i < 8; ++i)
             if (fabsf(x[j][r][i]) > kFinite) x[j][r][i] = copysignf(scale * 127.0f, x[j][r][i]);
     }
-    int8_t* tile = codes + sc * page * DIM;
     if (mine && scale > before && lo > 0) {  // older tokens of the page move to the larger scale
       const float f = __fdiv_rn(before, scale);
       for (int i = tid; i < lo * (DIM / 8); i += per_head) {
-        uint2* at = reinterpret_cast<uint2*>(tile) + i;
+        uint2* at = reinterpret_cast<uint2*>(codes + sc * page * DIM) + i;
         const uint2 w = *at;
         float y[8];
 #pragma unroll
@@ -335,8 +345,9 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
     }
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
-      if (!mine || slot[j] < lo || slot[j] >= hi) continue;
-      int8_t* o = tile + slot[j] * DIM;
+      int8_t* o = to[j];
+      to[j] += (size_t)groups * page * DIM;
+      if (!mine || !in[j]) continue;
       const uint2 c0 = codes8(x[j][0], unit), c1 = codes8(x[j][1], unit);
       if (at1[j] == at0[j] + 8) {
         *reinterpret_cast<uint4*>(o + at0[j]) = make_uint4(c0.x, c0.y, c1.x, c1.y);
@@ -347,6 +358,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
     }
     // every thread has read the old scale before the barrier above
     if (mine && tid == 0) scales[sc] = scale;
+    sc += groups;
   }
   // new tokens past the last page slot of the grid
   if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1 && (g + 1) * (long long)page < sv.len)
