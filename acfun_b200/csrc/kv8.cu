@@ -117,13 +117,21 @@ struct AppendArgs {
   int head_block;  // heads of one block
 };
 
-// The larger of a and |b|; NaN when either is.
+// The larger of |a| and |b|, of either sign; NaN when either is.
 __device__ __forceinline__ float amax_nan(float a, float b) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// The same over a warp.
+// x / 127 rounded to nearest: the quotient by the rounded reciprocal, corrected once by its exact
+// remainder (Markstein's theorem on division with fused multiply-add; x is far from both ends of
+// the range).
+__device__ __forceinline__ float div127(float x) {
+  constexpr float y = 1.0f / 127.0f;
+  const float q = __fmul_rn(x, y);
+  return __fmaf_rn(__fmaf_rn(-127.0f, q, x), y, q);
+}
+// The largest over a warp.
 __device__ __forceinline__ float warp_max_nan(float a) {
   float d;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
@@ -227,6 +235,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   const T* from[UN];  // of the next head to request
   int8_t* to[UN];     // of the head at hand
   size_t sc = (size_t)pid * a.kv.heads + h0 + group;
+  const long long from_step = groups * head_stride, to_step = (long long)groups * page * DIM;
 #pragma unroll
   for (int j = 0; j < UN; ++j) {
     in[j] = slot[j] >= lo && slot[j] < hi;
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[j][0].u[i] = raw[j][1].u[i] = make_uint4(0, 0, 0, 0);
       }
-      from[j] += groups * head_stride;
+      from[j] += from_step;
     }
   };
   request(h0 + group);
@@ -297,7 +306,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
         for (int i = 0; i < 8; ++i) top = amax_nan(top, x[j][r][i]);
     }
     // the head's maximum; the buffers alternate so that one barrier per round is enough
-    top = warp_max_nan(top);
+    top = warp_max_nan(fabsf(top));
     if ((threadIdx.x & 31) == 0) warp_max[0][buf][threadIdx.x >> 5] = top;
     __syncthreads();
     const int lane = threadIdx.x & 31;
@@ -321,7 +330,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
       __syncthreads();
       for (int w = w0; w < w1; ++w) top = fmaxf(top, warp_max[1][buf][w]);
     }
-    const float scale = fmaxf(before, __fdiv_rn(top, 127.0f));
+    const float scale = fmaxf(before, div127(top));
     const float unit = __frcp_rn(scale);
     if (__builtin_expect(!finite, 0)) {
 #pragma unroll
@@ -346,7 +355,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
       int8_t* o = to[j];
-      to[j] += (size_t)groups * page * DIM;
+      to[j] += to_step;
       if (!mine || !in[j]) continue;
       const uint2 c0 = codes8(x[j][0], unit), c1 = codes8(x[j][1], unit);
       if (at1[j] == at0[j] + 8) {
