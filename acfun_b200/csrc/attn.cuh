@@ -181,9 +181,13 @@ struct AttnArgs {
   int dtype, q_heads, group;  // group = q_heads / kv.heads
   float scale;
   int causal, window;
+  // sequences whose rows (new tokens * group) are within [rows_least, rows_most] are this launch's
+  long long rows_least, rows_most;
 };
+__device__ __forceinline__ bool rows_taken(const AttnArgs& a, int rows) {
+  return rows >= a.rows_least && rows <= a.rows_most;
+}
 bool attn_stream_dev(Call& c, const AttnArgs& a);  // any shape
-bool attn_tc_dev(Call& c, const AttnArgs& a);      // where attn_tc_takes
-bool attn_tc_takes(const AttnArgs& a);
+bool attn_tc_dev(Call& c, const AttnArgs& a);      // dim 64 or 128
 
 }  // namespace acf

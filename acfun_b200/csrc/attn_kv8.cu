@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
   const SeqView sv = seq_view(a.b, seq, err);
   const int rows = sv.n * a.group;
   const int r0 = rt * RT;
-  if (r0 >= rows) return;
+  if (r0 >= rows || !rows_taken(a, rows)) return;
   const int nr = min(RT, rows - r0);
   const int t_first = r0 / a.group, t_last = (r0 + nr - 1) / a.group;
   const int pos0 = sv.len - sv.n;  // position of new token 0 (negative: it sees nothing)
@@ -465,38 +465,90 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
   __syncthreads();
   if (!sm.last) return;
   __threadfence();
-  constexpr int PL = DIM / 32;  // elements per lane
-  for (int r = warp; r < nr; r += kWarps) {  // a warp per row, 32 chunks at a time
+  // All (row, chunk) offsets and sums are requested at once and kept in shared memory, in blocks of
+  // chunks if they are many; then a thread takes 4 elements of some rows, all chunks of which are
+  // again independent loads.  A round trip to L2 takes longer than everything else here.
+  float2* ml = reinterpret_cast<float2*>(sm.o);  // [row][chunk of the block]
+  const int kb = min(nsplit, (int)(sizeof(sm.o) / sizeof(float2)) / nr);
+  auto row_at = [&](int r) -> size_t {
     const int t = (r0 + r) / a.group, hq = head * a.group + (r0 + r) - t * a.group;
-    const size_t at = ((size_t)(sv.row0 + t) * a.q_heads + hq) * p.splits;
-    float top = -INFINITY;
-    for (int k = lane; k < nsplit; k += 32) top = fmaxf(top, __ldcg(&p.part_ml[at + k]).x);
+    return ((size_t)(sv.row0 + t) * a.q_heads + hq) * p.splits;
+  };
+  auto fetch_ml = [&](int k0) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < nr * kb; i += blockDim.x) {
+      const int r = i / kb, k = k0 + i - r * kb;
+      ml[i] = k < nsplit ? __ldcg(&p.part_ml[row_at(r) + k]) : make_float2(-INFINITY, 0.0f);
+    }
+    __syncthreads();
+  };
+  for (int r = threadIdx.x; r < RT; r += blockDim.x) sm.row_ml[r][0] = -INFINITY, sm.row_ml[r][1] = 0.0f;
+  for (int k0 = 0; k0 < nsplit; k0 += kb) {  // the rows' largest offsets
+    fetch_ml(k0);
+    for (int r = warp; r < nr; r += kWarps) {
+      float top = sm.row_ml[r][0];
+      for (int k = lane; k < kb; k += 32) top = fmaxf(top, ml[r * kb + k].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float x[PL] = {}, sum = 0.0f;
-    for (int k0 = 0; k0 < nsplit; k0 += 32) {
-      const int n = min(32, nsplit - k0);
-      const float2 ml = lane < n ? __ldcg(&p.part_ml[at + k0 + lane]) : make_float2(-INFINITY, 0.0f);
-      const float mine = lane < n ? (ml.x == top ? 1.0f : ex2(ml.x - top)) : 0.0f;
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float b = __shfl_sync(0xffffffffu, mine, k);
-        sum = fmaf(__shfl_sync(0xffffffffu, ml.y, k), b, sum);
-        const float* v = p.part_o + (at + k0 + k) * DIM + lane * PL;
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) sm.row_ml[r][0] = top;
+    }
+  }
+  constexpr int kItems = RT * DIM / 4 / (kWarps * 32);
+  float4 acc[kItems];
+  const float* from[kItems];
+  int row[kItems];
 #pragma unroll
-        for (int e = 0; e < PL; e += 2) {
-          const float2 w = __ldcg(reinterpret_cast<const float2*>(v + e));
-          x[e] = fmaf(w.x, b, x[e]), x[e + 1] = fmaf(w.y, b, x[e + 1]);
+  for (int j = 0; j < kItems; ++j) {
+    const int i = threadIdx.x + j * kWarps * 32;
+    row[j] = i / (DIM / 4);
+    from[j] = p.part_o + row_at(min(row[j], nr - 1)) * DIM + 4 * (i % (DIM / 4));
+    acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  for (int k0 = 0; k0 < nsplit; k0 += kb) {
+    if (kb < nsplit)
+      fetch_ml(k0);
+    else
+      __syncthreads();
+    for (int r = warp; r < nr; r += kWarps) {  // the sums make way for the chunks' factors
+      const float top = sm.row_ml[r][0];
+      float sum = 0.0f;
+      for (int k = lane; k < kb; k += 32) {
+        float2& x = ml[r * kb + k];
+        const float b = x.x == top ? 1.0f : ex2(x.x - top);
+        sum = fmaf(x.y, b, sum);
+        x.y = b;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) sm.row_ml[r][1] += sum;
+    }
+    __syncthreads();
+    const int n = min(kb, nsplit - k0);
+#pragma unroll(kItems >= 8 ? 2 : 16 / kItems)
+    for (int k = 0; k < n; ++k) {
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        if (row[j] < nr) {
+          const float b = ml[row[j] * kb + k].y;
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(from[j] + (size_t)(k0 + k) * DIM));
+          acc[j].x = fmaf(v.x, b, acc[j].x), acc[j].y = fmaf(v.y, b, acc[j].y);
+          acc[j].z = fmaf(v.z, b, acc[j].z), acc[j].w = fmaf(v.w, b, acc[j].w);
         }
       }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* dst = out + (long long)(sv.row0 + t) * a.o_token + (long long)hq * a.o_head + lane * PL;
+  }
 #pragma unroll
-    for (int e = 0; e < PL; e += 2) store2(dst + e, x[e] * inv, x[e + 1] * inv);
-    if (lane == 0 && a.lse)
+  for (int j = 0; j < kItems; ++j) {
+    const int i = threadIdx.x + j * kWarps * 32, r = i / (DIM / 4), d = 4 * (i % (DIM / 4));
+    if (r >= nr) continue;
+    const int t = (r0 + r) / a.group, hq = head * a.group + (r0 + r) - t * a.group;
+    const float of = sm.row_ml[r][1], inv = of == 0.0f ? 0.0f : 1.0f / of;
+    T* dst = out + (long long)(sv.row0 + t) * a.o_token + (long long)hq * a.o_head + d;
+    store2(dst, acc[j].x * inv, acc[j].y * inv);
+    store2(dst + 2, acc[j].z * inv, acc[j].w * inv);
+    if (d == 0 && a.lse)
       a.lse[(long long)(sv.row0 + t) * a.q_heads + hq] =
-          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+          of == 0.0f ? -INFINITY : (sm.row_ml[r][0] + log2f(of)) * 0.69314718055994531f;
   }
 }
 
@@ -530,7 +582,7 @@ bool stream_launch(Call& c, const AttnArgs& a) {
   }
   StreamArgs p = {};
   p.a = a;
-  const long long tiles = ((long long)std::min(a.b.max_new, a.b.tokens) * a.group + 8 * R8 - 1) / (8 * R8);
+  const long long tiles = (std::min(std::min(a.b.max_new, a.b.tokens) * (long long)a.group, a.rows_most) + 8 * R8 - 1) / (8 * R8);
   if (tiles * a.kv.heads > 0x7fffffffLL) {
     set_error(kInvalid, "acfun_kv8_attention: too many rows");
     return false;
@@ -578,7 +630,7 @@ template <typename T, int DIM>
 bool stream_rows(Call& c, const AttnArgs& a) {
   // the widest tile that the rows fill: each tile reads (from L2, after the first) and converts the
   // keys again.  32 rows of 256 elements do not fit in the registers.
-  const long long rows = (long long)std::min(a.b.max_new, a.b.tokens) * a.group;
+  const long long rows = std::min(std::min(a.b.max_new, a.b.tokens) * (long long)a.group, a.rows_most);
   if (rows <= 8) return stream_launch<T, DIM, 1>(c, a);
   if (rows <= 16 || DIM == 256) return stream_launch<T, DIM, 2>(c, a);
   return stream_launch<T, DIM, DIM == 256 ? 2 : 4>(c, a);
@@ -619,6 +671,10 @@ extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatc
     set_error(kInvalid, "%s: window %d must not be negative and needs causal", what, window);
     return kInvalid;
   }
+  if ((long long)std::min(batch->max_new, tokens) * (q_heads / cache->heads) > 0x3fffffffLL) {
+    set_error(kInvalid, "%s: max_new %d new tokens of %d heads are too many rows", what, batch->max_new, q_heads);
+    return kInvalid;
+  }
   if (int e = check_strides(what, q_token, q_head, tokens, q_heads, dim, false)) return e;
   if (int e = check_strides(what, o_token, o_head, tokens, q_heads, dim, true)) return e;
   if (batch->seqs == 0 || tokens == 0 || batch->max_new == 0) return 0;
@@ -638,6 +694,23 @@ extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatc
   a.q_token = q_token, a.q_head = q_head, a.o_token = o_token, a.o_head = o_head;
   a.dtype = dtype, a.q_heads = q_heads, a.group = q_heads / cache->heads;
   a.scale = scale, a.causal = causal != 0, a.window = window;
-  if (!(attn_tc_takes(a) ? attn_tc_dev(c, a) : attn_stream_dev(c, a))) c.fail();
+  // Sequences with more than 32 rows per cache head go to the tensor cores' tiles of 128, the others are
+  // streamed.  Measured with 32 query and 8 cache heads of 128 elements, 16 sequences of 4096 keys:
+  // 16 rows 56 us streamed and 88 us tiled, 32 rows 80 and 84, 64 rows 132 and 85.  A batch may hold
+  // both kinds (decode steps beside prompts); where every sequence has max_new tokens it does not.
+  constexpr long long kStreamRows = 32;
+  const long long most = std::min(batch->max_new, tokens) * (long long)a.group;
+  const bool tiled = most > kStreamRows && dim != 256;
+  const bool streamed = !tiled || (batch->seqs > 1 && a.group <= kStreamRows && tokens < (long long)batch->seqs * batch->max_new);
+  bool ok = true;
+  if (tiled) {
+    a.rows_least = streamed ? kStreamRows + 1 : 0, a.rows_most = 0x7fffffffLL;
+    ok = attn_tc_dev(c, a);
+  }
+  if (ok && streamed) {
+    a.rows_least = 0, a.rows_most = tiled ? kStreamRows : 0x7fffffffLL;
+    ok = attn_stream_dev(c, a);
+  }
+  if (!ok) c.fail();
   return c.finish() ? 0 : last_error_code();
 }

@@ -50,7 +50,7 @@ constexpr int kStep = 64;      // keys of one S product and its softmax
 constexpr int kUnits = kKeys / 16;
 constexpr int kFmaOf4 = 1;      // pairs of four whose 2^x the FMA units compute instead of the special function unit
 constexpr float kLeast = 1e-37f;  // a factor never underflows to 0: a masked score stays -inf under it
-constexpr int kPreRowTiles = 3;
+constexpr int kPreRowTiles = 24;
 constexpr size_t kPreBytes = size_t(1) << 30;
 constexpr int kScaleRing = 4;  // the converters are at most two tiles ahead of a softmax
 
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(256) k_kv8_tiles(const TcArgs p, unsigned* err
   const AttnArgs& a = p.a;
   const int tile = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
   const SeqView sv = seq_view(a.b, seq, err);
-  if (sv.n == 0) return;
+  if (sv.n == 0 || !rows_taken(a, sv.n * a.group)) return;
   const KeyRange kr = key_range(a, sv, 0, sv.n * a.group, kKeys);
   if (tile < kr.first || tile >= kr.first + kr.n) return;
   const int v = threadIdx.x >> 7, t = threadIdx.x & 127;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
   const int seq = blockIdx.y, part = blockIdx.z;
   const SeqView sv = seq_view(a.b, seq, err);
   const int rows = sv.n * a.group, r0 = rt * kRows;
-  if (r0 >= rows) return;
+  if (r0 >= rows || !rows_taken(a, rows)) return;
   const int nr = min(kRows, rows - r0);
   const KeyRange kr = key_range(a, sv, r0, nr, kKeys);
   const int nsplit = max(1, (kr.n + p.chunk - 1) / p.chunk);
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
       int rr = r0 + t * 128 + w0 + sub;
       int h = rr % a.group;
       const T* src = q + (long long)(sv.row0 + rr / a.group) * a.q_token + (long long)(head * a.group + h) * a.q_head + c * 8;
-#pragma unroll 1
+#pragma unroll 4
       for (int i = 0; i < N; ++i) {
         if (rr < rows) {
           if (vec) {
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const TcArgs p, unsigned* err
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, seq = blockIdx.y;
   const SeqView sv = seq_view(a.b, seq, err);
-  if (item >= (long long)sv.n * a.q_heads) return;
+  if (item >= (long long)sv.n * a.q_heads || !rows_taken(a, sv.n * a.group)) return;
   const int tok = (int)(item / a.q_heads), hq = (int)(item - (long long)tok * a.q_heads);
   const int r = tok * a.group + hq % a.group, r0 = r / kRows * kRows;
   const KeyRange kr = key_range(a, sv, r0, min(kRows, sv.n * a.group - r0), kKeys);
@@ -814,11 +814,6 @@ bool tc_run(Call& c, const AttnArgs& a) {
 bool attn_tc_dev(Call& c, const AttnArgs& a) {
   if (a.dtype == ACFUN_F16) return a.kv.dim == 64 ? tc_run<__half, 64>(c, a) : tc_run<__half, 128>(c, a);
   return a.kv.dim == 64 ? tc_run<__nv_bfloat16, 64>(c, a) : tc_run<__nv_bfloat16, 128>(c, a);
-}
-
-bool attn_tc_takes(const AttnArgs& a) {
-  const long long rows = (long long)std::min(a.b.max_new, a.b.tokens) * a.group;
-  return (a.kv.dim == 64 || a.kv.dim == 128) && rows > 64 && rows * a.kv.heads < (1LL << 31);
 }
 
 }  // namespace acf
