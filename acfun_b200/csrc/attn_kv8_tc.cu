@@ -523,64 +523,54 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
     float q_unit = 1.0f;
     {
       // Q to shared memory: a warp copies its 32 rows as they are, all in flight at once, DIM / 8 lanes
-      // with 16 bytes of a row each.  Where K is fp16 whatever q is, the rows are then converted in
-      // place, each scaled by a power of two.
+      // with 16 bytes of a row each; a row's place in memory comes from the lane that owns the row.
       constexpr int LPR = DIM / 8, RPP = 32 / LPR, N = 32 / RPP;  // lanes per row, rows per pass, passes
       const int sub = lane / LPR, c = lane % LPR;
       const T* q = static_cast<const T*>(a.q);
       const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && a.q_token % 8 == 0 && a.q_head % 8 == 0;
-      const int w0 = (warp & 3) * 32;  // first row of the warp in its tile
-      uint8_t* tile = smem + L::kQ + t * L::kQTile + (c >> 3) * (128 * 128);
-      auto place = [&](int i) -> uint8_t* {
-        const int r = w0 + i * RPP + sub;
-        return tile + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-      };
-      int rr = r0 + t * 128 + w0 + sub;
-      int h = rr % a.group;
-      const T* src = q + (long long)(sv.row0 + rr / a.group) * a.q_token + (long long)(head * a.group + h) * a.q_head + c * 8;
+      const long long own = in ? (long long)(sv.row0 + tok) * a.q_token + (long long)hq * a.q_head : -1;
+      uint8_t* tile = smem + L::kQ + t * L::kQTile;
+      uint8_t* at = tile + (c >> 3) * (128 * 128) + ((warp & 3) * 32 + sub) * 128;
 #pragma unroll 4
       for (int i = 0; i < N; ++i) {
-        if (rr < rows) {
-          if (vec) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dev::smem_u32(place(i))), "l"(src) : "memory");
-          } else {
-            T* o = reinterpret_cast<T*>(place(i));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = src[e];
-          }
+        const long long from = __shfl_sync(0xffffffffu, own, i * RPP + sub);
+        uint8_t* to = at + i * RPP * 128 + (((c & 7) ^ ((i * RPP + sub) & 7)) << 4);
+        if (from < 0) {
+          *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+        } else if (vec) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dev::smem_u32(to)), "l"(q + from + c * 8) : "memory");
         } else {
-          *reinterpret_cast<uint4*>(place(i)) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(to)[e] = q[from + c * 8 + e];
         }
-        rr += RPP, h += RPP, src += RPP * a.q_head;
-        while (h >= a.group) h -= a.group, src += a.q_token - a.group * a.q_head;
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      if constexpr (!PRE) {  // each lane converts what it copied itself
+      // Where K is fp16 and q is not (or the scale's sign has to go somewhere), each thread converts its
+      // row in place, scaled by a power of two.
+      if (!PRE && (!std::is_same<T, __half>::value || a.scale < 0.0f)) {
+        __syncwarp();
+        uint8_t* mine = tile + row * 128;
+        float top = 0.0f;
 #pragma unroll 4
-      for (int i = 0; i < N; ++i) {
-        uint4* at = reinterpret_cast<uint4*>(place(i));
-        union {
-          uint4 u;
-          T e[8];
-        } x;
-        x.u = *at;
-        float y[8], top = 0.0f;
+        for (int k = 0; k < DIM / 8; ++k) {
+          float x[8];
+          load8(reinterpret_cast<const T*>(mine + (k >> 3) * (128 * 128) + (((k & 7) ^ (row & 7)) << 4)), true, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = to_f(x.e[e]), top = fmaxf(top, fabsf(y[e]));
-#pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        }
         const Pow2 f = row_pow2(top);
         const float down = copysignf(f.down, a.scale);
-#pragma unroll
-        for (int k = 0; k < RPP; ++k) {
-          const float up = __shfl_sync(0xffffffffu, f.up, k * LPR);
-          if (lane == i * RPP + k) q_unit = up;
+        q_unit = f.up;
+#pragma unroll 4
+        for (int k = 0; k < DIM / 8; ++k) {
+          uint8_t* p16 = mine + (k >> 3) * (128 * 128) + (((k & 7) ^ (row & 7)) << 4);
+          float x[8];
+          load8(reinterpret_cast<const T*>(p16), true, x);
+          uint4 o;
+          o.x = pack_f16(x[0] * down, x[1] * down), o.y = pack_f16(x[2] * down, x[3] * down);
+          o.z = pack_f16(x[4] * down, x[5] * down), o.w = pack_f16(x[6] * down, x[7] * down);
+          *reinterpret_cast<uint4*>(p16) = o;
         }
-        uint4 o;
-        o.x = pack_f16(y[0] * down, y[1] * down), o.y = pack_f16(y[2] * down, y[3] * down);
-        o.z = pack_f16(y[4] * down, y[5] * down), o.w = pack_f16(y[6] * down, y[7] * down);
-        *at = o;
-      }
       }
       dev::fence_proxy_async_smem();
       arrive(&bar.q_full);
@@ -677,9 +667,10 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
       const bool none = ntiles == 0 || (m == -INFINITY && l == l);
       const float inv = none ? 0.0f : 1.0f / l;
       const bool whole = nsplit == 1;
-      T* dst = static_cast<T*>(a.out) + (long long)(sv.row0 + tok) * a.o_token + (long long)hq * a.o_head;
-      const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
       const size_t at = ((size_t)(sv.row0 + tok) * a.q_heads + hq) * p.splits + part;
+      // A thread has a row, but 32 rows at a time are 32 places in memory: the rows go through this
+      // tile's part of Q, which no product needs any more, and leave DIM / 8 lanes to a row.
+      uint8_t* stage = smem + L::kQ + t * L::kQTile + row * 128;
 #pragma unroll 1
       for (int i = 0; i < DIM / 32; ++i) {
         float o[32];
@@ -690,19 +681,43 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.0f;
         }
-        if (!in || !ok) continue;
+        if (!ok) continue;
         if (whole) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             float x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = none ? 0.0f : o[e + k] * inv;
-            store8(dst + i * 32 + e, vec, x);
+            const int k16 = i * 4 + e / 8;
+            store8(reinterpret_cast<T*>(stage + (k16 >> 3) * (128 * 128) + (((k16 & 7) ^ (row & 7)) << 4)), true, x);
           }
-        } else {
+        } else if (in) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(p.part_o + at * DIM + i * 32 + e) = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            *reinterpret_cast<float4*>(p.part_o + at * DIM + i * 32 + e) =
+                none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      if (whole && ok) {
+        constexpr int LPR = DIM / 8, RPP = 32 / LPR;
+        const int sub = lane / LPR, c = lane % LPR;
+        T* out = static_cast<T*>(a.out);
+        const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && a.o_token % 8 == 0 && a.o_head % 8 == 0;
+        const long long own = in ? (long long)(sv.row0 + tok) * a.o_token + (long long)hq * a.o_head : -1;
+        const uint8_t* from = smem + L::kQ + t * L::kQTile + (c >> 3) * (128 * 128) + ((warp & 3) * 32 + sub) * 128;
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < 32 / RPP; ++i) {
+          const long long to = __shfl_sync(0xffffffffu, own, i * RPP + sub);
+          if (to < 0) continue;
+          const uint4 w = *reinterpret_cast<const uint4*>(from + i * RPP * 128 + (((c & 7) ^ ((i * RPP + sub) & 7)) << 4));
+          if (vec) {
+            *reinterpret_cast<uint4*>(out + to + c * 8) = w;
+          } else {
+            const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[to + c * 8 + e] = x[e];
+          }
         }
       }
       if (in && ok) {
@@ -778,8 +793,9 @@ bool tc_run(Call& c, const AttnArgs& a) {
   const long long work = (long long)p.row_tiles * a.kv.heads * a.b.seqs;
   const int tiles = (a.b.max_len + kKeys - 1) / kKeys;
   const long long want = std::max<long long>(1, c.sm_count() / std::max<long long>(1, work));
-  p.chunk = (int)std::max<long long>(4, (tiles + 1 + want - 1) / want);
-  p.splits = (tiles + 1 + p.chunk - 1) / p.chunk;  // a window can start inside a tile
+  const int most = tiles + (a.window > 0);  // a window can start inside a tile
+  p.chunk = (int)std::max<long long>(4, (most + want - 1) / want);
+  p.splits = (most + p.chunk - 1) / p.chunk;
   if (p.splits > 1) {
     const size_t n = (size_t)a.b.tokens * a.q_heads * p.splits;
     p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
