@@ -442,27 +442,51 @@ __global__ void __launch_bounds__(256) k_kv8_read(const ReadArgs a, unsigned* er
   const int rows = hi - lo, total = nh * rows * CPR;
   const size_t head0 = (size_t)pid * a.kv.heads + h0;
   const long long out0 = (long long)(sv.row0 + g * page + lo - first) * a.kv.heads + h0;
-  for (int i = threadIdx.x; i < total; i += blockDim.x) {
-    const int c = i % CPR, rest = i / CPR, r = rest % rows, h = rest / rows;
-    const size_t from = (((head0 + h) * page) + lo + r) * DIM + 16 * c;
-    const size_t to = (size_t)(out0 + (long long)r * a.kv.heads + h) * DIM + 16 * c;
-    uint4 wk = {}, wv = {};
-    float sk = 0.f, sv_ = 0.f;
-    if (a.k) wk = *reinterpret_cast<const uint4*>(a.kv.k + from), sk = a.kv.ks[head0 + h];
-    if (a.v) wv = *reinterpret_cast<const uint4*>(a.kv.v + from), sv_ = a.kv.vs[head0 + h];
+  constexpr int U = 2;  // runs under way per thread, of K and of V each
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 31) == 0;
+  for (int i0 = threadIdx.x; i0 < total; i0 += U * blockDim.x) {
+    uint4 w[U][2];
+    float scale[U][2];
+    size_t to[U];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      T* o = static_cast<T*>(which ? a.v : a.k);
-      if (!o) continue;
-      const uint4 w = which ? wv : wk;
-      const float s = which ? sv_ : sk;
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * (int)blockDim.x, total - 1);
+      const int c = i % CPR, rest = i / CPR, h = nh == 1 ? 0 : rest / rows, r = rest - h * rows;
+      const size_t from = (((head0 + h) * page) + lo + r) * DIM + 16 * c;
+      to[u] = (size_t)(out0 + (long long)r * a.kv.heads + h) * DIM + 16 * c;
+      if (a.k) w[u][0] = __ldg(reinterpret_cast<const uint4*>(a.kv.k + from)), scale[u][0] = a.kv.ks[head0 + h];
+      if (a.v) w[u][1] = __ldg(reinterpret_cast<const uint4*>(a.kv.v + from)), scale[u][1] = a.kv.vs[head0 + h];
+    }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x[8];
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * (int)blockDim.x >= total) break;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = code_value(words[2 * e + j / 4] ^ 0x80808080u, j % 4) * s;
-        store8(o + to + 8 * e, true, x);
+      for (int which = 0; which < 2; ++which) {
+        T* o = static_cast<T*>(which ? a.v : a.k);
+        if (!o) continue;
+        const uint32_t words[4] = {w[u][which].x, w[u][which].y, w[u][which].z, w[u][which].w};
+        if (wide) {  // 32 bytes per store: a whole sector per lane
+          union {
+            T t[32 / sizeof(T)];
+            uint32_t w[8];
+          } y;
+          constexpr int E = 32 / (int)sizeof(T);
+#pragma unroll
+          for (int e = 0; e < 16; e += E) {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+              y.t[j] = from_f<T>(code_value(words[(e + j) / 4] ^ 0x80808080u, j % 4) * scale[u][which]);
+            dev::st_global_v8(o + to[u] + e, y.w);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = code_value(words[(e + j) / 4] ^ 0x80808080u, j % 4) * scale[u][which];
+            store8(o + to[u] + e, true, x);
+          }
+        }
       }
     }
   }
