@@ -177,7 +177,7 @@ int acfun_set_fp32_math(int mode);
 #define ACFUN_F16 1
 #define ACFUN_BF16 2
 
-/* Codes [pages][heads][page][dim] and one scale per (page, head): value = code * scale.
+/* Codes [pages][heads][page][dim] and one positive scale per (page, head): value = code * scale.
  * page is 16, 32, 64 or 128 tokens; dim is 64, 128 or 256. */
 typedef struct AcfunKvCache8 {
   int8_t* k;
