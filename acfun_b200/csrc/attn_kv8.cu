@@ -589,7 +589,7 @@ bool stream_launch(Call& c, const AttnArgs& a) {
   }
   p.row_tiles = (int)tiles;
   // Split the keys so that one wave of resident blocks covers the batch.  Sequences of a batch may
-  // differ in length: chunks of about 1024 keys keep the longest from being the last (48 ragged
+  // differ in length: chunks of at most about 2048 keys keep the longest from being the last (48 ragged
   // sequences: 512 keys 73 us, 1024 and 2048 59 us), longer ones only where these would make more
   // than 16 waves of blocks.  Blocks that walk a list of the chunks there are, made from the lengths
   // in the kernel, took 61 us: their start has to wait for the list.
@@ -597,7 +597,7 @@ bool stream_launch(Call& c, const AttnArgs& a) {
   const long long slots = (long long)per_sm[dv] * c.sm_count();
   const long long want = std::max<long long>(1, slots / std::max<long long>(1, work));
   long long chunk = (a.b.max_len + want - 1) / want;
-  if (a.b.seqs > 1) chunk = std::min(chunk, std::max<long long>(1024, work * a.b.max_len / (16 * slots)));
+  if (a.b.seqs > 1) chunk = std::min(chunk, std::max<long long>(2048, work * a.b.max_len / (16 * slots)));
   chunk = std::max<long long>(chunk, kUnit * kPair * kWarps);
   chunk = std::min<long long>((chunk + kUnit - 1) / kUnit * kUnit, (long long)(kMaxPages - 1) * a.kv.page);
   p.chunk = (int)chunk;
