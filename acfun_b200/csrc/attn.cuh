@@ -183,11 +183,13 @@ struct AttnArgs {
   int causal, window;
   // sequences whose rows (new tokens * group) are within [rows_least, rows_most] are this launch's
   long long rows_least, rows_most;
+  bool beside;  // the launch before in the stream is k_attn_tc of the same call
 };
 __device__ __forceinline__ bool rows_taken(const AttnArgs& a, int rows) {
   return rows >= a.rows_least && rows <= a.rows_most;
 }
 bool attn_stream_dev(Call& c, const AttnArgs& a);  // any shape
-bool attn_tc_dev(Call& c, const AttnArgs& a);      // dim 64 or 128
+// dim 64 or 128; *last_is_main: whether its last launch is k_attn_tc
+bool attn_tc_dev(Call& c, const AttnArgs& a, bool* last_is_main);
 
 }  // namespace acf

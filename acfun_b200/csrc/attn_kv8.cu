@@ -128,7 +128,7 @@ static_assert(alignof(StreamSmem<64, 1>) == 128 && alignof(Ring<64>) == 128 && s
 
 // DIM / 64 runs of 16 bytes per key for K; DIM / 8 bytes per key for V.
 template <typename T, int DIM, int R8>
-__global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_stream(const StreamArgs p, unsigned* err) {
+__device__ __forceinline__ void attn_stream(const StreamArgs& p, unsigned* err) {
   constexpr int KR = DIM / 64;          // 16-byte runs of a thread per key (K)
   constexpr int MT = DIM / 16;          // output m-tiles
   constexpr int VW = DIM / 32;          // 32-bit words of a thread per key (V)
@@ -136,8 +136,6 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
   extern __shared__ __align__(128) uint8_t smem_raw[];
   using Smem = StreamSmem<DIM, R8>;
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-  dev::grid_dep_wait();
-  dev::grid_dep_launch();
   const AttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int head = blockIdx.x % a.kv.heads, rt = blockIdx.x / a.kv.heads, seq = blockIdx.y, chunk_i = blockIdx.z;
@@ -552,6 +550,16 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
   }
 }
 
+template <typename T, int DIM, int R8>
+__global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_stream(const StreamArgs p, unsigned* err) {
+  // Beside k_attn_tc the kernel before is not a producer but the other half of the same call: what it
+  // waited for is complete, and only the end waits for it, so that completion stays in order.
+  if (!p.a.beside) dev::grid_dep_wait();
+  dev::grid_dep_launch();
+  attn_stream<T, DIM, R8>(p, err);
+  if (p.a.beside) dev::grid_dep_wait();
+}
+
 // Zeroed once per device; the kernel leaves it zero.
 unsigned* tickets_of(int device) {
   static unsigned* buf[64] = {};
@@ -705,7 +713,7 @@ extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatc
   bool ok = true;
   if (tiled) {
     a.rows_least = streamed ? kStreamRows + 1 : 0, a.rows_most = 0x7fffffffLL;
-    ok = attn_tc_dev(c, a);
+    ok = attn_tc_dev(c, a, &a.beside);
   }
   if (ok && streamed) {
     a.rows_least = 0, a.rows_most = tiled ? kStreamRows : 0x7fffffffLL;

@@ -254,6 +254,9 @@ template <typename T, int DIM, bool PRE>
 __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArgs p, unsigned* err) {
   using L = TcSmem<DIM>;
   extern __shared__ uint8_t smem_raw[];
+  // Launched normally: everything before it in the stream is complete.  Once every block has started,
+  // the streaming kernel of the same call may run on the SMs that are free.
+  dev::grid_dep_launch();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcBars& bar = *reinterpret_cast<TcBars*>(smem + L::kBars);
   float4* scales = reinterpret_cast<float4*>(smem + L::kScales);  // [ring][unit]: k factor, log2 v, 1 / v
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
       const long long own = in ? (long long)(sv.row0 + tok) * a.q_token + (long long)hq * a.q_head : -1;
       uint8_t* tile = smem + L::kQ + t * L::kQTile;
       uint8_t* at = tile + (c >> 3) * (128 * 128) + ((warp & 3) * 32 + sub) * 128;
-#pragma unroll 4
+#pragma unroll 8
       for (int i = 0; i < N; ++i) {
         const long long from = __shfl_sync(0xffffffffu, own, i * RPP + sub);
         uint8_t* to = at + i * RPP * 128 + (((c & 7) ^ ((i * RPP + sub) & 7)) << 4);
@@ -671,7 +674,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
       // A thread has a row, but 32 rows at a time are 32 places in memory: the rows go through this
       // tile's part of Q, which no product needs any more, and leave DIM / 8 lanes to a row.
       uint8_t* stage = smem + L::kQ + t * L::kQTile + row * 128;
-#pragma unroll 1
+#pragma unroll 2
       for (int i = 0; i < DIM / 32; ++i) {
         float o[32];
         if (ntiles > 0) {
@@ -706,7 +709,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
         const long long own = in ? (long long)(sv.row0 + tok) * a.o_token + (long long)hq * a.o_head : -1;
         const uint8_t* from = smem + L::kQ + t * L::kQTile + (c >> 3) * (128 * 128) + ((warp & 3) * 32 + sub) * 128;
         __syncwarp();
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < 32 / RPP; ++i) {
           const long long to = __shfl_sync(0xffffffffu, own, i * RPP + sub);
           if (to < 0) continue;
@@ -784,7 +787,7 @@ bool tc_launch(Call& c, TcArgs p, dim3 grid) {
 }
 
 template <typename T, int DIM>
-bool tc_run(Call& c, const AttnArgs& a) {
+bool tc_run(Call& c, const AttnArgs& a, bool* last_is_main) {
   TcArgs p = {};
   p.a = a;
   const long long max_new = std::min(a.b.max_new, a.b.tokens);
@@ -817,6 +820,7 @@ bool tc_run(Call& c, const AttnArgs& a) {
   } else if (!tc_launch<T, DIM, false>(c, p, grid)) {
     return false;
   }
+  *last_is_main = p.splits == 1;
   if (p.splits > 1) {
     const long long items = (max_new * a.q_heads + 3) / 4;
     k_attn_join<T, DIM><<<dim3((unsigned)items, a.b.seqs), 128, 0, c.stream()>>>(p, c.err());
@@ -827,9 +831,9 @@ bool tc_run(Call& c, const AttnArgs& a) {
 
 }  // namespace
 
-bool attn_tc_dev(Call& c, const AttnArgs& a) {
-  if (a.dtype == ACFUN_F16) return a.kv.dim == 64 ? tc_run<__half, 64>(c, a) : tc_run<__half, 128>(c, a);
-  return a.kv.dim == 64 ? tc_run<__nv_bfloat16, 64>(c, a) : tc_run<__nv_bfloat16, 128>(c, a);
+bool attn_tc_dev(Call& c, const AttnArgs& a, bool* last_is_main) {
+  if (a.dtype == ACFUN_F16) return a.kv.dim == 64 ? tc_run<__half, 64>(c, a, last_is_main) : tc_run<__half, 128>(c, a, last_is_main);
+  return a.kv.dim == 64 ? tc_run<__nv_bfloat16, 64>(c, a, last_is_main) : tc_run<__nv_bfloat16, 128>(c, a, last_is_main);
 }
 
 }  // namespace acf
