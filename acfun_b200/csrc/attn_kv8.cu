@@ -1,6 +1,7 @@
 // attn_kv8.cu — attention over the int8 cache (acfun_kv8_attention): the entry point and the
-// streaming kernel, whose warps turn codes straight into matrix-instruction fragments.  It takes any shape; attention with few rows per cache head (decode steps, drafts)
-// is bound by the codes it reads, and that is what it is built for.
+// streaming kernel, whose warps turn codes straight into matrix-instruction fragments.  It takes any
+// shape; attention with few rows per cache head (decode steps, drafts) is bound by the codes it
+// reads, and that is what it is built for.
 //
 // Rows: the new tokens of a sequence times the query heads that share a cache head, row = token *
 // group + head, in tiles of 8, 16 or 32.  A block of four warps takes one (sequence, cache head, row
@@ -25,6 +26,11 @@
 // is 16 consecutive bytes (8 when dim is 64); the weights change from C to B operand by movmatrix.
 // The codes pass through a ring in shared memory of two steps of 32 keys per warp, copied
 // asynchronously; nothing is shared between warps.
+//
+// Measured (B200): one fp16 token of 64 query heads over 262145 keys of 8 cache heads of 128 elements
+// 100 us, 5.4 TB/s, 82 % of the measured copy rate, at 1.65 GHz under the board's power limit; one
+// token each of 48 sequences of 33 to 16000 keys, 32 query and 8 cache heads, 56 us, 4.0 TB/s, where
+// blocks that find no chunk of their own and the joins of short chunks cost the rest.
 #include <math.h>
 
 #include <algorithm>

@@ -2,25 +2,34 @@
 // rows per cache head (prompts, chunks of prompts, batches of drafts).
 //
 // Rows are packed as in attn_kv8.cu (row = token * group + head of the group), 256 to a block: two
-// tiles of 128, A and B, against the same keys.  Per 128 keys and tile
-//   S = Q K^T  (M = 128, N = 128, both operands fp16 in shared memory)  -> TMEM
+// tiles of 128, A and B, against the same keys.  Per 64 keys and tile
+//   S = Q K^T  (M = 128, N = 64, both operands in shared memory)  -> TMEM
 //   w = 2^(S f + log2 s_v - m) in registers, one row per thread, rounded to fp16 -> TMEM, over S
 //   O += w V   (A operand from TMEM, V's codes as fp16 in shared memory, N = dim)  -> TMEM
-// so the tensor cores work on one tile while the other is in its softmax.  Codes are exact in fp16;
-// K scales, V scales and q's power of two enter the exponent as in attn_kv8.cu, and the running
-// offset m moves only when a weight would pass 2^15, so O is rescaled a few times per row at most.
+// so the tensor cores work on one tile while the other is in its softmax.  Codes are exact in fp16
+// (and bf16); K and V scales enter the exponent as in attn_kv8.cu, and the running offset m moves
+// only when a weight would pass 2^15, so O is rescaled a few times per row at most.
 //
 //   warps 0-3, 4-7  Q of tile A / B to shared memory, then its softmax and output (a TMEM lane and
 //                   a row per thread)
-// The codes become fp16 in the 128-byte swizzled layout of the MMA operands in one of two places:
-//   in the kernel   warps 8-11 convert the block's keys one tile ahead (two stages each for K and V),
-//                   warps 12 and 13 issue the MMAs; the cache is read once per 256 rows, at one byte a code
-//   before it       k_kv8_tiles writes each key tile's image to scratch once, and warp 10 only copies
-//                   images (cp.async.bulk), warps 8 and 9 issue the MMAs.  Conversion costs the softmax's
-//                   issue slots and registers, and with many row tiles it is repeated for each.
-// TMEM: two buffers of S of A and of B (64 keys, 64 columns each; the fp16 weights overlay their
-// first half), O of A and B.  With one buffer of 128 keys a softmax waited a third of its time for
-// the products between its weights and its next scores.
+// The codes become 16-bit operands in the MMA's 128-byte swizzled layout in one of two places:
+//   in the kernel   warps 8-11 convert the block's keys one tile of 128 ahead (two stages each for K and
+//                   V), warps 12 and 13 issue the MMAs; the cache is read once per 256 rows, at a byte
+//                   a code.  K is fp16, and q is brought to fp16 by a power of two per row.
+//   before it       k_kv8_tiles writes each key tile's image to scratch once, warp 10 only copies images
+//                   (cp.async.bulk), warps 8 and 9 issue the MMAs.  K takes q's type.  Conversion costs the
+//                   softmax's issue slots and registers, and with many row tiles it is repeated for each.
+// TMEM: two buffers of S of A and of B (64 columns each; the fp16 weights overlay their first half),
+// O of A and B.  With one buffer of 128 keys a softmax waited a third of its time for the products
+// between its weights and its next scores.
+//
+// Measured (B200, 32 query and 8 cache heads of 128 elements, bf16, causal): a prompt of 8192 tokens
+// 535 us, 1.03 PFLOP/s of what the mask leaves, 63 % of the measured bf16 peak, at 1.65 GHz under the
+// board's power limit.  A step of 64 keys of both tiles takes about 1650 cycles; its products need
+// 1280, its 2^x 770 of the special function units (a quarter of them on the FMA units: none 1.22 and
+// half 1.11 times as long per softmax), and it issues 880 instructions per scheduler.  Two threads per
+// row, with four softmax warps per scheduler instead of two, took 565 us: the exchange of maxima cost
+// more than the latencies it hid.
 // Every wait is bounded (ptx.cuh); on expiry the error word is set and all roles leave.
 #include <math.h>
 
@@ -50,6 +59,9 @@ constexpr int kStep = 64;      // keys of one S product and its softmax
 constexpr int kUnits = kKeys / 16;
 constexpr int kFmaOf4 = 1;      // pairs of four whose 2^x the FMA units compute instead of the special function unit
 constexpr float kLeast = 1e-37f;  // a factor never underflows to 0: a masked score stays -inf under it
+// Row tiles from which the key tiles are converted before the kernel (32 query, 8 cache heads of 128:
+// 16 row tiles 34.5 us converted in the kernel and 35.0 us before it, 32 row tiles 60.6 and 55.5), and
+// the most scratch that this may take.
 constexpr int kPreRowTiles = 24;
 constexpr size_t kPreBytes = size_t(1) << 30;
 constexpr int kScaleRing = 4;  // the converters are at most two tiles ahead of a softmax

@@ -404,6 +404,34 @@ def test_host_activations(acf):
     P.check_attention(torch.from_numpy(got), None, [t.cpu() for t in P.attention64(cache, b, torch.from_numpy(q).cuda(), 64 ** -0.5, True, 0)], "f16")
 
 
+def test_offsets_past_32_bits(acf):
+    """A cache of 2.3 GB of codes each for keys and values, whose last pages are the ones in use."""
+    pages, heads, page, dim = 70000, 8, 64, 64
+    assert pages * heads * page * dim > 2 ** 31
+    codes = [torch.empty((pages, heads, page, dim), dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.full((pages, heads), 0.01, device="cuda") for _ in range(2)]
+    cache = acf.KvCache8(*codes, *scales)
+    for new, length in (([3, 1], [3, 700]), ([100, 1], [650, 40])):
+        b = P.Batch(acf, new, length, page, seed=33, spare_pages=0)
+        b.table = torch.where(b.table >= 0, pages - 1 - b.table, b.table)
+        b.dev[0].copy_(b.table)
+        for codes_of in (cache.k, cache.v):   # what is in the cache already
+            used = b.table[b.table >= 0].long().cuda()
+            codes_of[used] = torch.randint(-127, 128, (len(used), heads, page, dim), device="cuda").to(torch.int8)
+        kv = randn(34, b.tokens, 2, heads, dim).to(torch.bfloat16)
+        q = randn(35, b.tokens, 2 * heads, dim).to(torch.bfloat16)
+        cache.append(kv[:, 0], kv[:, 1], b.h)
+        k, _ = cache.read(b.h, torch.float32)
+        got = cache.attention(q, b.h, scale=0.1)
+        acf.synchronize()
+        for i in range(2):
+            rows = slice(b.start[i], b.start[i + 1])
+            want = b.whole(cache.k, cache.k_scale, i)[b.length[i] - b.new[i]:]
+            assert torch.equal(k[rows].double(), want.float().double())
+            assert ((want - kv[rows, 0].double()).abs() <= cache.k_scale[b.table[i, 0].item()].max().double() * 4).all()
+        P.check_attention(got, None, P.attention64(cache, b, q, 0.1, True, 0), "bf16")
+
+
 # ------------------------------------------------------------------ bad device data is reported, not read
 def test_bad_entries_are_reported(acf):
     b = P.Batch(acf, [2, 2, 40], [40, 50, 60], 16, seed=2)
