@@ -31,6 +31,16 @@ def _dtype_code(dt):
     return code
 
 
+_calls = {}  # the library's functions by name, bound at their first use
+
+
+def _fn(name):
+    f = _calls.get(name)
+    if f is None:
+        f = _calls[name] = getattr(lib(), name)
+    return f
+
+
 class _Cache(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
                 ("pages", C.c_int), ("heads", C.c_int), ("page", C.c_int), ("dim", C.c_int)]
@@ -56,25 +66,43 @@ def _flat(x, code, what):
     return _address(x)
 
 
-def _strides(x, what):
-    """(token, head) strides in elements of [tokens, heads, dim]."""
-    if x.ndim != 3:
-        raise ValueError(f"{what} must be [tokens, heads, dim], got {tuple(x.shape)}")
+def _rows(x, what):
+    """(address, dtype code, shape, token stride, head stride) of [tokens, heads, dim]; strides in
+    elements."""
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"{what} must be [tokens, heads, dim], got {tuple(shape)}")
     if isinstance(x, np.ndarray):
         t, h, d = (s // x.itemsize for s in x.strides)
+        at = x.ctypes.data
     else:
         t, h, d = x.stride()
-    if d != 1 and x.shape[2] != 1:
+        at = x.data_ptr()
+    if d != 1 and shape[2] != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous")
-    return t, h
+    return at, _dtype_code(x.dtype), shape, t, h
 
 
-def _like(x):
-    """An uninitialised array of x's shape and dtype, where x is."""
-    if isinstance(x, np.ndarray):
-        return np.empty(x.shape, x.dtype)
-    import torch
-    return torch.empty_like(x)
+_empty_like = None  # torch's, once a torch tensor has come by
+
+
+def _out(out, x, shape, code, what):
+    """(out, address, token stride, head stride) of an output like x, made when it is None."""
+    if out is None and not isinstance(x, np.ndarray):
+        global _empty_like
+        if _empty_like is None:
+            from torch import empty_like as _empty_like
+        out = _empty_like(x)
+        t, h, d = out.stride()
+        if d == 1 or shape[2] == 1:
+            return out, out.data_ptr(), t, h
+        out = out.contiguous()  # x's dimensions overlap or repeat
+    elif out is None:
+        out = np.empty(shape, x.dtype)
+    at, out_code, out_shape, t, h = _rows(out, "out")
+    if out_shape != shape or out_code != code:
+        raise ValueError(f"out must have {what}'s shape and dtype")
+    return out, at, t, h
 
 
 def _done(code):
@@ -108,24 +136,21 @@ def rope_frequencies(rot, base=10000.0, scaling=None, factor=1.0, trained=0, fas
         raise ValueError("rot must be positive")
     freq = np.empty(rot // 2, np.float32)
     amp = C.c_float()
-    _done(lib().acfun_rope_frequencies(rot, base, kinds[scaling], factor, trained, fast, slow, freq.ctypes.data,
+    _done(_fn("acfun_rope_frequencies")(rot, base, kinds[scaling], factor, trained, fast, slow, freq.ctypes.data,
                                        C.byref(amp)))
     return freq, amp.value
 
 
 def rope(x, positions, spec: Rope, out=None):
     """x [tokens, heads, dim] at int32 positions [tokens]; out may be x."""
-    t, h = _strides(x, "x")
-    tokens, heads, dim = x.shape
+    at, code, shape, t, h = _rows(x, "x")
+    tokens, heads, dim = shape
     if positions.shape != (tokens,):
         raise ValueError("positions must be [tokens]")
-    if out is None:
-        out = _like(x)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError("out must have x's shape and dtype")
-    ot, oh = _strides(out, "out")
-    _done(lib().acfun_rope(_address(x), _address(out), _dtype_code(x.dtype), tokens, heads, dim, t, h, ot, oh,
-                           _flat(positions, _I32, "positions"), spec.ref))
+    out, out_at, ot, oh = _out(out, x, shape, code, "x")
+    err = _fn("acfun_rope")(at, out_at, code, tokens, heads, dim, t, h, ot, oh, _flat(positions, _I32, "positions"), spec.ref)
+    if err:
+        _done(err)
     return out
 
 
@@ -169,41 +194,44 @@ class KvCache8:
         return cls(*codes, *scales)
 
     def _new(self, x, batch, what):
-        if tuple(x.shape) != (batch.tokens, self.heads, self.dim):
-            raise ValueError(f"{what} must be [{batch.tokens}, {self.heads}, {self.dim}], got {tuple(x.shape)}")
-        return _strides(x, what)
+        rows = _rows(x, what)
+        if rows[2] != (batch.tokens, self.heads, self.dim):
+            raise ValueError(f"{what} must be [{batch.tokens}, {self.heads}, {self.dim}], got {tuple(rows[2])}")
+        return rows
 
     def append(self, k, v, batch: KvBatch, rope: Rope | None = None):
         """Quantise the batch's new keys (rotated by their position in the sequence when rope is
         given) and values into their pages."""
-        kt, kh = self._new(k, batch, "k")
-        vt, vh = self._new(v, batch, "v")
-        if k.dtype != v.dtype:
+        k_at, code, _, kt, kh = self._new(k, batch, "k")
+        v_at, v_code, _, vt, vh = self._new(v, batch, "v")
+        if code != v_code:
             raise ValueError("k and v must have one dtype")
-        _done(lib().acfun_kv8_append(self.ref, batch.ref, _address(k), _address(v), _dtype_code(k.dtype), kt, kh, vt,
-                                     vh, rope.ref if rope is not None else None))
+        err = _fn("acfun_kv8_append")(self.ref, batch.ref, k_at, v_at, code, kt, kh, vt, vh,
+                                      rope.ref if rope is not None else None)
+        if err:
+            _done(err)
 
     def read(self, batch: KvBatch, dtype):
         """(k, v) [tokens, heads, dim]: the last start[i + 1] - start[i] tokens of each sequence."""
+        code = _dtype_code(dtype)
         k, v = self.k.new_empty((2, batch.tokens, self.heads, self.dim), dtype=dtype).unbind()
-        _done(lib().acfun_kv8_read(self.ref, batch.ref, k.data_ptr(), v.data_ptr(), _dtype_code(dtype)))
+        err = _fn("acfun_kv8_read")(self.ref, batch.ref, k.data_ptr(), v.data_ptr(), code)
+        if err:
+            _done(err)
         return k, v
 
     def attention(self, q, batch: KvBatch, scale=None, causal=True, window=0, out=None, lse=None):
         """softmax(scale * q k^T) v for q [tokens, q_heads, dim]; scale defaults to dim ** -0.5.  lse
         (fp32 [tokens, q_heads]) receives the logarithm of the softmax denominators."""
-        qt, qh = _strides(q, "q")
-        if q.shape[0] != batch.tokens or q.shape[2] != self.dim:
-            raise ValueError(f"q must be [{batch.tokens}, q_heads, {self.dim}], got {tuple(q.shape)}")
-        if out is None:
-            out = _like(q)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out must have q's shape and dtype")
-        if lse is not None and tuple(lse.shape) != tuple(q.shape[:2]):
+        at, code, shape, qt, qh = _rows(q, "q")
+        if shape[0] != batch.tokens or shape[2] != self.dim:
+            raise ValueError(f"q must be [{batch.tokens}, q_heads, {self.dim}], got {tuple(shape)}")
+        if lse is not None and tuple(lse.shape) != tuple(shape[:2]):
             raise ValueError("lse must be [tokens, q_heads]")
-        ot, oh = _strides(out, "out")
-        _done(lib().acfun_kv8_attention(self.ref, batch.ref, _address(q), _address(out), _dtype_code(q.dtype),
-                                        q.shape[1], qt, qh, ot, oh, self.dim ** -0.5 if scale is None else scale,
-                                        int(bool(causal)), window,
-                                        _flat(lse, _F32, "lse") if lse is not None else None))
+        out, out_at, ot, oh = _out(out, q, shape, code, "q")
+        err = _fn("acfun_kv8_attention")(self.ref, batch.ref, at, out_at, code, shape[1], qt, qh, ot, oh,
+                                         self.dim ** -0.5 if scale is None else scale, int(bool(causal)), window,
+                                         _flat(lse, _F32, "lse") if lse is not None else None)
+        if err:
+            _done(err)
         return out
