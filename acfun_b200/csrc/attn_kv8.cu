@@ -145,6 +145,10 @@ __device__ __forceinline__ void attn_stream(const StreamArgs& p, unsigned* err) 
   const AttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int head = blockIdx.x % a.kv.heads, rt = blockIdx.x / a.kv.heads, seq = blockIdx.y, chunk_i = blockIdx.z;
+  const int lg = a.kv.page_log2;
+  // without a window the chunk's pages do not depend on the length: their numbers come with it
+  const int guess = (int)(((long long)chunk_i * p.chunk) >> lg) + threadIdx.x;
+  const int early = a.window == 0 && guess < a.b.cols ? __ldg(a.b.table + (size_t)seq * a.b.cols + guess) : -1;
   const SeqView sv = seq_view(a.b, seq, err);
   const int rows = sv.n * a.group;
   const int r0 = rt * RT;
@@ -160,10 +164,16 @@ __device__ __forceinline__ void attn_stream(const StreamArgs& p, unsigned* err) 
   const int ub = unit0 + chunk_i * per, ue = min(unit0 + units, ub + per);
 
   // the chunk's pages
-  const int lg = a.kv.page_log2;
   const int pg0 = (ub * kUnit) >> lg;
   const int npg = ue > ub ? (((ue * kUnit - 1) >> lg) - pg0 + 1) : 0;
-  for (int i = threadIdx.x; i < npg; i += blockDim.x) sm.pages[i].pid = seq_page(a.b, seq, pg0 + i, a.kv.pages, err);
+  for (int i = threadIdx.x; i < npg; i += blockDim.x) {
+    int pid = a.window == 0 && i == (int)threadIdx.x ? early : a.b.table[(size_t)seq * a.b.cols + pg0 + i];
+    if ((unsigned)pid >= (unsigned)a.kv.pages) {
+      atomicOr(err, ACF_DEV_ERR_BADARG);
+      pid = -1;
+    }
+    sm.pages[i].pid = pid;
+  }
   __syncthreads();
 
   const size_t head_at = (size_t)head * a.kv.page, page_step = (size_t)a.kv.heads * a.kv.page;

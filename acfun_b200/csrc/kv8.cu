@@ -185,28 +185,9 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   if (g * (long long)page >= sv.len) return;
   const int lo = max(first - g * page, 0), hi = min(sv.len - g * page, page);  // new slots [lo, hi)
   const int row_of_slot0 = sv.row0 + g * page - first;  // packed row of slot 0 (may be before row0)
-  const int pid = seq_page(a.b, seq, g, a.kv.pages, err);
-  if (pid < 0) return;
   const int h0 = (blockIdx.y >> 1) * a.head_block, h1 = min(h0 + a.head_block, a.kv.heads);
   const int half = a.rot / 2;
   const bool turn = !is_v && a.rot > 0;
-  if (turn) {
-    // A thread takes a pair's run of consecutive tokens: the first angle is computed, the others
-    // are turned on from it by one position's angle (at most 127 turns, each within 2^-23).
-    const int n = hi - lo, runs = max(1, (int)blockDim.x / half), len = (n + runs - 1) / runs;
-    for (int i = threadIdx.x; i < half * runs; i += blockDim.x) {
-      const int t0 = i / half * len, pair = i % half;
-      if (t0 >= n) continue;
-      const float f = a.freq[pair];
-      float2 w = rope_cs(g * page + lo + t0, f, a.amp);
-      const float2 one = len > 1 ? rope_cs(1, f, 1.0f) : make_float2(1.0f, 0.0f);
-      for (int t = t0; t < min(t0 + len, n); ++t) {
-        cs[t * half + pair] = w;
-        w = make_float2(w.x * one.x - w.y * one.y, w.y * one.x + w.x * one.y);
-      }
-    }
-    __syncthreads();
-  }
   const int per_head = page * DIM / (16 * UN), group = threadIdx.x / per_head, groups = blockDim.x / per_head;
   const int tid = threadIdx.x - group * per_head;
   // this thread's units: slot and the element offsets of their two runs
@@ -241,13 +222,11 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   bool in[UN];
   const T* from[UN];  // of the next head to request
   int8_t* to[UN];     // of the head at hand
-  size_t sc = (size_t)pid * a.kv.heads + h0 + group;
   const long long from_step = groups * head_stride, to_step = (long long)groups * page * DIM;
 #pragma unroll
   for (int j = 0; j < UN; ++j) {
     in[j] = slot[j] >= lo && slot[j] < hi;
     from[j] = src + (long long)(row_of_slot0 + slot[j]) * tok_stride + (h0 + group) * head_stride;
-    to[j] = codes + sc * page * DIM + slot[j] * DIM;
   }
   auto request = [&](int h) {
 #pragma unroll
@@ -262,7 +241,30 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
       from[j] += from_step;
     }
   };
+  // the first values, the page's number and the angles are on their way together
   request(h0 + group);
+  const int pid = seq_page(a.b, seq, g, a.kv.pages, err);
+  if (pid < 0) return;
+  size_t sc = (size_t)pid * a.kv.heads + h0 + group;
+#pragma unroll
+  for (int j = 0; j < UN; ++j) to[j] = codes + sc * page * DIM + slot[j] * DIM;
+  if (turn) {
+    // A thread takes a pair's run of consecutive tokens: the first angle is computed, the others
+    // are turned on from it by one position's angle (at most 127 turns, each within 2^-23).
+    const int n = hi - lo, runs = max(1, (int)blockDim.x / half), len = (n + runs - 1) / runs;
+    for (int i = threadIdx.x; i < half * runs; i += blockDim.x) {
+      const int t0 = i / half * len, pair = i % half;
+      if (t0 >= n) continue;
+      const float f = a.freq[pair];
+      float2 w = rope_cs(g * page + lo + t0, f, a.amp);
+      const float2 one = len > 1 ? rope_cs(1, f, 1.0f) : make_float2(1.0f, 0.0f);
+      for (int t = t0; t < min(t0 + len, n); ++t) {
+        cs[t * half + pair] = w;
+        w = make_float2(w.x * one.x - w.y * one.y, w.y * one.x + w.x * one.y);
+      }
+    }
+    __syncthreads();
+  }
   for (int hb = h0, buf = 0; hb < h1; hb += groups, buf ^= 1) {
     const bool mine = hb + group < h1;  // a group without a head of its own only keeps the barriers
     float x[UN][2][8];
