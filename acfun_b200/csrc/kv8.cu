@@ -122,6 +122,7 @@ struct AppendArgs {
   int rot, interleaved;
   float amp;
   int head_block;  // heads of one block
+  int per_head;    // threads of one head: whole warps, enough for the new tokens that a page can get
 };
 
 // The larger of |a| and |b|, of either sign; NaN when either is.
@@ -160,8 +161,9 @@ template <int DIM>
 constexpr int kUnits = DIM == 256 ? 2 : 1;
 
 // One block: page slot blockIdx.x of the new tokens of sequence blockIdx.z, heads
-// [blockIdx.y / 2 * head_block, ...), keys (blockIdx.y even) or values (odd).  A head takes page * DIM
-// / 16 threads, so that small pages have several heads in a block at a time.  A thread holds a
+// [blockIdx.y / 2 * head_block, ...), keys (blockIdx.y even) or values (odd).  A head takes the threads
+// that a page's share of max_new tokens needs, so that small pages and single tokens have several
+// heads in a block at a time.  A thread holds a
 // unit of 16 elements of the tile (two of them when dim is 256) in registers between the maximum and
 // the coding: two runs of 8 elements, which in the half layout are the two sides of 8 pairs.
 template <typename T, int DIM>
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   const int h0 = (blockIdx.y >> 1) * a.head_block, h1 = min(h0 + a.head_block, a.kv.heads);
   const int half = a.rot / 2;
   const bool turn = !is_v && a.rot > 0;
-  const int per_head = page * DIM / (16 * UN), group = threadIdx.x / per_head, groups = blockDim.x / per_head;
+  const int per_head = a.per_head, group = threadIdx.x / per_head, groups = blockDim.x / per_head;
   const int tid = threadIdx.x - group * per_head;
   // this thread's units: slot and the element offsets of their two runs
   int slot[UN], at0[UN], at1[UN], cs_at[UN];
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   for (int j = 0; j < UN; ++j) {
     const int idx = tid + j * per_head;
     const int u = idx % UPR;
-    slot[j] = idx / UPR;
+    slot[j] = lo + idx / UPR;
     cs_at[j] = -1;
     if (turn && !a.interleaved) {
       const int pairs = a.rot / 16;
@@ -386,14 +388,15 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
 template <typename T, int DIM>
 bool append_launch(Call& c, AppendArgs a) {
   const int page = a.kv.page;
-  const int per_head = page * DIM / (16 * kUnits<DIM>);
+  const int per_head = (std::min(page, a.b.max_new) * DIM / (16 * kUnits<DIM>) + 31) / 32 * 32;
+  a.per_head = per_head;
   // pages that a run of max_new tokens can touch
   const int slots = std::max(1, (std::min(a.b.max_new, a.b.max_len) + page - 2) / page + 1);
   // All heads of a page in one block share its cosines and sines; with few pages the heads go to
   // blocks of their own, which recompute them but fill the machine.
   const long long pages = (long long)slots * a.b.seqs;
   int parts = (int)std::min<long long>(a.kv.heads, std::max<long long>(1, 4LL * c.sm_count() / std::max<long long>(1, pages)));
-  a.head_block = (a.kv.heads + parts - 1) / parts;
+  a.head_block = std::min(a.kv.heads, std::max((a.kv.heads + parts - 1) / parts, 128 / per_head));
   parts = (a.kv.heads + a.head_block - 1) / a.head_block;
   const int threads = per_head * std::max(1, std::min(a.head_block, 256 / per_head));
   const size_t smem = (size_t)std::min(page, a.b.max_new) * (a.rot / 2) * sizeof(float2);
