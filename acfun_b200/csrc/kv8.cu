@@ -117,7 +117,7 @@ struct AppendArgs {
   const void* k;
   const void* v;
   long long k_token, k_head, v_token, v_head;
-  int k_vec, v_vec;
+  int vec;  // k and v can be read 16 bytes at a time
   const float* freq;
   int rot, interleaved;
   float amp;
@@ -166,7 +166,7 @@ constexpr int kUnits = DIM == 256 ? 2 : 1;
 // heads in a block at a time.  A thread holds a
 // unit of 16 elements of the tile (two of them when dim is 256) in registers between the maximum and
 // the coding: two runs of 8 elements, which in the half layout are the two sides of 8 pairs.
-template <typename T, int DIM>
+template <typename T, int DIM, bool VEC>
 __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigned* err) {
   extern __shared__ __align__(16) float2 cs[];  // [tokens in this page][rot / 2], keys only
   __shared__ float warp_max[2][2][32];
@@ -215,7 +215,6 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   }
   const T* src = static_cast<const T*>(is_v ? a.v : a.k);
   const long long tok_stride = is_v ? a.v_token : a.k_token, head_stride = is_v ? a.v_head : a.k_head;
-  const bool vec = is_v ? a.v_vec : a.k_vec;
   int8_t* codes = is_v ? a.kv.v : a.kv.k;
   float* scales = is_v ? a.kv.vs : a.kv.ks;
 
@@ -234,8 +233,8 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
       if (h < h1 && in[j]) {
-        load8_raw(from[j] + at0[j], vec, raw[j][0]);
-        load8_raw(from[j] + at1[j], vec, raw[j][1]);
+        load8_raw(from[j] + at0[j], VEC, raw[j][0]);
+        load8_raw(from[j] + at1[j], VEC, raw[j][1]);
       } else {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[j][0].u[i] = raw[j][1].u[i] = make_uint4(0, 0, 0, 0);
@@ -385,8 +384,8 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
     atomicOr(err, ACF_DEV_ERR_BADARG);
 }
 
-template <typename T, int DIM>
-bool append_launch(Call& c, AppendArgs a) {
+template <typename T, int DIM, bool VEC>
+bool append_run(Call& c, AppendArgs a) {
   const int page = a.kv.page;
   const int per_head = (std::min(page, a.b.max_new) * DIM / (16 * kUnits<DIM>) + 31) / 32 * 32;
   a.per_head = per_head;
@@ -403,15 +402,19 @@ bool append_launch(Call& c, AppendArgs a) {
   static bool attr_done[64] = {false};
   const int dv = current_device();
   if (smem > 48 * 1024 && !attr_done[dv & 63]) {
-    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_kv8_append<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_kv8_append<T, DIM, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           128 * (DIM / 2) * (int)sizeof(float2))))
       return false;
     attr_done[dv & 63] = true;
   }
-  if (!ACF_CUDA_OK(launch_pdl(k_kv8_append<T, DIM>, dim3(slots, 2 * parts, a.b.seqs), dim3(threads), smem, c.stream(), a,
+  if (!ACF_CUDA_OK(launch_pdl(k_kv8_append<T, DIM, VEC>, dim3(slots, 2 * parts, a.b.seqs), dim3(threads), smem, c.stream(), a,
                               c.err())))
     return false;
   return c.launched("k_kv8_append");
+}
+template <typename T, int DIM>
+bool append_launch(Call& c, const AppendArgs& a) {
+  return a.vec ? append_run<T, DIM, true>(c, a) : append_run<T, DIM, false>(c, a);
 }
 
 // ------------------------------------------------------------------ read
@@ -568,8 +571,8 @@ extern "C" int acfun_kv8_append(const AcfunKvCache8* cache, const AcfunKvBatch* 
   }
   if (!c.ok()) return last_error_code();
   const long long per16 = 16 / (long long)dtype_size(dtype);
-  a.k_vec = aligned16(a.k) && k_token % per16 == 0 && k_head % per16 == 0;
-  a.v_vec = aligned16(a.v) && v_token % per16 == 0 && v_head % per16 == 0;
+  a.vec = aligned16(a.k) && k_token % per16 == 0 && k_head % per16 == 0 && aligned16(a.v) && v_token % per16 == 0 &&
+          v_head % per16 == 0;
   a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
   if (!ACF_BY_DTYPE(append_launch, dtype, a)) c.fail();
   return c.finish() ? 0 : last_error_code();
