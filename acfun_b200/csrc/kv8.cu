@@ -157,6 +157,20 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float unit) {
                     __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
+// n words of 8 codes, coded under `before`, moved to `scale`.  Out of line, so that what it needs is not
+// prepared for every head.
+__device__ __noinline__ void move_codes(int8_t* codes, int n, float before, float scale, int tid, int threads) {
+  const float f = __fdiv_rn(before, scale);
+  uint2* w = reinterpret_cast<uint2*>(codes);
+  for (int i = tid; i < n; i += threads) {
+    const uint2 v = w[i];
+    float y[8];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) y[b] = (float)(int8_t)(v.x >> (8 * b)), y[4 + b] = (float)(int8_t)(v.y >> (8 * b));
+    w[i] = codes8(y, f);
+  }
+}
+
 template <int DIM>
 constexpr int kUnits = DIM == 256 ? 2 : 1;
 
@@ -351,16 +365,8 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
           for (int i = 0; i < 8; ++i)
             if (fabsf(x[j][r][i]) > kFinite) x[j][r][i] = copysignf(scale * 127.0f, x[j][r][i]);
     }
-    if (mine && scale > before && lo > 0) {  // older tokens of the page move to the larger scale
-      const float f = __fdiv_rn(before, scale);
-      for (int i = tid; i < lo * (DIM / 8); i += per_head) {
-        uint2* at = reinterpret_cast<uint2*>(codes + sc * page * DIM) + i;
-        const uint2 w = *at;
-        float y[8];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) y[b] = (float)(int8_t)(w.x >> (8 * b)), y[4 + b] = (float)(int8_t)(w.y >> (8 * b));
-        *at = codes8(y, f);
-      }
+    if (__builtin_expect(lo > 0, 0)) {  // older tokens of the page move to a larger scale
+      if (mine && scale > before) move_codes(to[0] - slot[0] * DIM, lo * (DIM / 8), before, scale, tid, per_head);
     }
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
