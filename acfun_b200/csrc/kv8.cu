@@ -157,6 +157,10 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float unit) {
                     __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
+// Place of pair i in a token's row of cosines and sines: 8 pairs (a unit's) stay together, their four
+// 16-byte quarters exchanged so that eight neighbouring units read 128 different bytes at a time.
+__device__ __forceinline__ int cs_place(int i) { return (i & ~6) | ((((i >> 1) ^ (i >> 4)) & 3) << 1); }
+
 // n words of 8 codes, coded under `before`, moved to `scale`.  Out of line, so that what it needs is not
 // prepared for every head.
 __device__ __noinline__ void move_codes(int8_t* codes, int n, float before, float scale, int tid, int threads) {
@@ -207,13 +211,13 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
   const int per_head = a.per_head, group = threadIdx.x / per_head, groups = blockDim.x / per_head;
   const int tid = threadIdx.x - group * per_head;
   // this thread's units: slot and the element offsets of their two runs
-  int slot[UN], at0[UN], at1[UN], cs_at[UN];
+  int slot[UN], at0[UN], at1[UN], cs_at[UN], cs_x[UN];
 #pragma unroll
   for (int j = 0; j < UN; ++j) {
     const int idx = tid + j * per_head;
     const int u = idx % UPR;
     slot[j] = lo + idx / UPR;
-    cs_at[j] = -1;
+    cs_at[j] = -1, cs_x[j] = (u >> 1) & 3;
     if (turn && !a.interleaved) {
       const int pairs = a.rot / 16;
       if (u < pairs) {
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
       float2 w = rope_cs(g * page + lo + t0, f, a.amp);
       const float2 one = len > 1 ? rope_cs(1, f, 1.0f) : make_float2(1.0f, 0.0f);
       for (int t = t0; t < min(t0 + len, n); ++t) {
-        cs[t * half + pair] = w;
+        cs[t * half + cs_place(pair)] = w;
         w = make_float2(w.x * one.x - w.y * one.y, w.y * one.x + w.x * one.y);
       }
     }
@@ -301,7 +305,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
           for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              const float4 c = w[(4 * r + i) / 2];
+              const float4 c = w[((4 * r + i) / 2) ^ cs_x[j]];
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 const float cc = k ? c.z : c.x, ss = k ? c.w : c.y;
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(1024) k_kv8_append(const AppendArgs a, unsigne
         } else {
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
-            const float4 c = w[i / 2];
+            const float4 c = w[(i / 2) ^ cs_x[j]];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const float cc = k ? c.z : c.x, ss = k ? c.w : c.y;
