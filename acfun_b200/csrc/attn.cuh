@@ -145,6 +145,10 @@ __device__ __forceinline__ float2 rope_cs(int pos, float f, float amp) {
   return make_float2(c * amp, s * amp);
 }
 
+// Place of pair i in a token's row of cosines and sines: 8 pairs (a thread's) stay together, their four
+// 16-byte quarters exchanged so that eight neighbouring threads read 128 different bytes at a time.
+__device__ __forceinline__ int cs_place(int i) { return (i & ~6) | ((((i >> 1) ^ (i >> 4)) & 3) << 1); }
+
 // ------------------------------------------------------------------ int8 -> fp16
 // Four signed bytes, XORed with 0x80808080, are u = code + 128; a byte u put under the exponent
 // byte 0x64 is the fp16 number 1024 + u, and subtracting 1152 is exact.

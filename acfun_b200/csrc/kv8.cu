@@ -157,10 +157,6 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float unit) {
                     __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
-// Place of pair i in a token's row of cosines and sines: 8 pairs (a unit's) stay together, their four
-// 16-byte quarters exchanged so that eight neighbouring units read 128 different bytes at a time.
-__device__ __forceinline__ int cs_place(int i) { return (i & ~6) | ((((i >> 1) ^ (i >> 4)) & 3) << 1); }
-
 // n words of 8 codes, coded under `before`, moved to `scale`.  Out of line, so that what it needs is not
 // prepared for every head.
 __device__ __noinline__ void move_codes(int8_t* codes, int n, float before, float scale, int tid, int threads) {

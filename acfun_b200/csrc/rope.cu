@@ -30,15 +30,15 @@ struct RopeArgs {
 // elements (interleaved, and what is copied); without VEC a pair or one copied element.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_rope(const RopeArgs a) {
-  extern __shared__ float2 cs[];  // [tok_block][rot / 2]
+  extern __shared__ __align__(16) float2 cs[];  // [tok_block][rot / 2 rounded up to 8], cs_place
   dev::grid_dep_wait();
   dev::grid_dep_launch();
-  const int half = a.rot / 2;
+  const int half = a.rot / 2, row = (half + 7) & ~7;
   const int t0 = blockIdx.x * a.tok_block, nt = min(a.tok_block, a.tokens - t0);
   const int h0 = blockIdx.y * a.head_block, nh = min(a.head_block, a.heads - h0);
   for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
     const int t = i / half;
-    cs[i] = rope_cs(a.pos[t0 + t], a.freq[i - t * half], a.amp);
+    cs[t * row + cs_place(i - t * half)] = rope_cs(a.pos[t0 + t], a.freq[i - t * half], a.amp);
   }
   __syncthreads();
   const T* x = static_cast<const T*>(a.x);
@@ -69,22 +69,32 @@ __global__ void __launch_bounds__(256) k_rope(const RopeArgs a) {
       for (int u = 0; u < U; ++u) {
         if (at[u] < 0) continue;
         if (at[u] < a.rot) {
-          const float2* w = cs + tok[u] * half;
+          // 8 pairs from a multiple of 8 (half), or 4 from a multiple of 4: quarters of a run of 8
+          const int p0 = a.interleaved ? at[u] / 2 : at[u], x = (p0 >> 4) & 3;
+          const float4* w = reinterpret_cast<const float4*>(cs + tok[u] * row + (p0 & ~7));
           if (a.interleaved) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 c = w[at[u] / 2 + i];
-              const float p = lo[u][2 * i], q = lo[u][2 * i + 1];
-              lo[u][2 * i] = p * c.x - q * c.y;
-              lo[u][2 * i + 1] = q * c.x + p * c.y;
+            for (int i = 0; i < 2; ++i) {
+              const float4 c = w[(((p0 & 7) >> 1) + i) ^ x];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float cc = k ? c.z : c.x, ss = k ? c.w : c.y;
+                const float p = lo[u][4 * i + 2 * k], q = lo[u][4 * i + 2 * k + 1];
+                lo[u][4 * i + 2 * k] = p * cc - q * ss;
+                lo[u][4 * i + 2 * k + 1] = q * cc + p * ss;
+              }
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 c = w[at[u] + i];
-              const float p = lo[u][i], q = hi[u][i];
-              lo[u][i] = p * c.x - q * c.y;
-              hi[u][i] = q * c.x + p * c.y;
+            for (int i = 0; i < 4; ++i) {
+              const float4 c = w[i ^ x];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float cc = k ? c.z : c.x, ss = k ? c.w : c.y;
+                const float p = lo[u][2 * i + k], q = hi[u][2 * i + k];
+                lo[u][2 * i + k] = p * cc - q * ss;
+                hi[u][2 * i + k] = q * cc + p * ss;
+              }
             }
             store8(y + dst[u] + half, true, hi[u]);
           }
@@ -98,7 +108,7 @@ __global__ void __launch_bounds__(256) k_rope(const RopeArgs a) {
       const T* p = x + (t0 + t) * a.x_token + (h0 + h) * a.x_head;
       T* o = y + (t0 + t) * a.y_token + (h0 + h) * a.y_head;
       if (j < half) {
-        const float2 c = cs[t * half + j];
+        const float2 c = cs[t * row + cs_place(j)];
         const int ia = a.interleaved ? 2 * j : j, ib = a.interleaved ? 2 * j + 1 : j + half;
         const float u = to_f(p[ia]), v = to_f(p[ib]);
         o[ia] = from_f<T>(u * c.x - v * c.y);
@@ -118,7 +128,7 @@ bool rope_launch(Call& c, RopeArgs a) {
   a.items = vec ? (a.interleaved ? a.dim / 8 : a.rot / 16 + (a.dim - a.rot) / 8) : a.rot / 2 + a.dim - a.rot;
   // tokens per block: enough blocks for about eight per SM; few tokens share their heads out
   const int want = 8 * c.sm_count();
-  int smem_cap = a.rot ? (40 * 1024) / (a.rot * 4) : 8;
+  int smem_cap = a.rot ? (40 * 1024) / (a.rot * 4 + 64) : 8;
   a.tok_block = std::max(1, std::min({a.tokens / want, 8, std::max(1, smem_cap)}));
   const int blocks = (a.tokens + a.tok_block - 1) / a.tok_block;
   int parts = std::max(1, std::min(a.heads, 2 * c.sm_count() / blocks));
@@ -130,7 +140,7 @@ bool rope_launch(Call& c, RopeArgs a) {
     set_error(kInvalid, "acfun_rope: too many heads");
     return false;
   }
-  const size_t smem = (size_t)a.tok_block * (a.rot / 2) * sizeof(float2);
+  const size_t smem = (size_t)a.tok_block * ((a.rot / 2 + 7) / 8 * 8) * sizeof(float2);
   if (!ACF_CUDA_OK(launch_pdl(vec ? k_rope<T, true> : k_rope<T, false>, dim3(blocks, parts), dim3(256), smem, c.stream(), a)))
     return false;
   return c.launched("k_rope");
