@@ -50,8 +50,9 @@ struct StreamArgs {
   AttnArgs a;
   int chunk;                 // keys per block, a multiple of kUnit
   int splits;                // chunks of max_len keys (the stride of the partial results)
-  float* part_o;             // [tokens][q_heads][splits][DIM], null when splits == 1
-  float2* part_ml;           // [tokens][q_heads][splits]
+  int part_rows;             // rows that a (sequence, head) of this launch can have
+  float* part_o;             // [seqs][heads][part_rows][splits][DIM], null when splits == 1
+  float2* part_ml;           // [seqs][heads][part_rows][splits]
   unsigned* tickets;         // [seqs][heads][row tiles], zero between calls
   int row_tiles;
 };
@@ -460,7 +461,7 @@ __device__ __forceinline__ void attn_stream(const StreamArgs& p, unsigned* err) 
         a.lse[(long long)(sv.row0 + t) * a.q_heads + hq] =
             sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
     } else {
-      const size_t at = ((size_t)(sv.row0 + t) * a.q_heads + hq) * p.splits + chunk_i;
+      const size_t at = (((size_t)seq * a.kv.heads + head) * p.part_rows + r0 + r) * p.splits + chunk_i;
       *reinterpret_cast<float2*>(p.part_o + at * DIM + d) = make_float2(x, y);
       if (d == 0) p.part_ml[at] = make_float2(top, sum);
     }
@@ -485,8 +486,7 @@ __device__ __forceinline__ void attn_stream(const StreamArgs& p, unsigned* err) 
   float2* ml = reinterpret_cast<float2*>(sm.o);  // [row][chunk of the block]
   const int kb = min(nsplit, (int)(sizeof(sm.o) / sizeof(float2)) / nr);
   auto row_at = [&](int r) -> size_t {
-    const int t = (r0 + r) / a.group, hq = head * a.group + (r0 + r) - t * a.group;
-    return ((size_t)(sv.row0 + t) * a.q_heads + hq) * p.splits;
+    return (((size_t)seq * a.kv.heads + head) * p.part_rows + r0 + r) * p.splits;
   };
   auto fetch_ml = [&](int k0) {
     __syncthreads();
@@ -632,7 +632,9 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     return false;
   }
   if (p.splits > 1) {
-    const size_t n = (size_t)a.b.tokens * a.q_heads * p.splits;
+    // by sequence, not by token: beside a prompt only the rows of the short sequences are here
+    p.part_rows = (int)std::min(std::min(a.b.max_new, a.b.tokens) * (long long)a.group, a.rows_most);
+    const size_t n = (size_t)a.b.seqs * a.kv.heads * p.part_rows * p.splits;
     p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
     p.part_ml = (float2*)c.scratch(n * sizeof(float2));
     if (work <= kTickets) {

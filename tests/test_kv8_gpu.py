@@ -18,7 +18,7 @@ ROPE = [  # dtype, tokens, heads, dim, rot, interleaved, largest position
     ("bf16", 1, 1, 64, 64, False, 10), ("f16", 7, 5, 128, 32, True, 100000), ("f32", 33, 3, 80, 20, False, 4000),
     ("f32", 300, 9, 64, 64, True, 1 << 30), ("bf16", 2100, 2, 128, 128, False, 131072), ("f16", 5, 3, 6, 6, True, 50),
     ("f32", 4, 2, 7, 4, False, 9), ("bf16", 3, 70, 256, 0, False, 9), ("f16", 2500, 3, 96, 48, False, 70000),
-    ("f32", 1300, 2, 72, 72, True, 70000)]
+    ("f32", 1300, 2, 72, 72, True, 70000), ("bf16", 9, 3, 192, 96, False, 5000), ("f16", 6, 2, 120, 104, True, 5000)]
 
 
 def check_rope(got, x, pos, freq, amp, inter, dtype):
@@ -125,7 +125,24 @@ def test_append_codes_and_scales_exactly(acf, dtype, heads, dim, page, new, leng
         assert np.array_equal(got[0].cpu().numpy(), codes)
 
 
-@pytest.mark.parametrize("inter,rot", [(False, 64), (True, 64), (False, 16), (True, 32), (False, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_append_from_unaligned_rows(acf, dtype):
+    """Keys and values one element off a 16-byte boundary, at odd strides; the cosines' path too."""
+    b = P.Batch(acf, [20, 1, 7], [33, 1, 40], 16, seed=3)
+    caches = [P.random_cache(acf, b.pages, 2, 64, 16, 4) for _ in range(2)]
+    freq = torch.from_numpy(acf.rope_frequencies(32)[0]).cuda()
+    for rope in (None, acf.Rope(freq), acf.Rope(freq, True)):
+        wide = randn(5, b.tokens * 301 + 1).to(P.DT[dtype])
+        kv = wide[1:].view(b.tokens, 301)[:, :256].unflatten(1, (2, 2, 64))
+        caches[0].append(kv[:, 0], kv[:, 1], b.h, rope=rope)
+        whole = kv.contiguous()
+        caches[1].append(whole[:, 0], whole[:, 1], b.h, rope=rope)
+        acf.synchronize()
+        for x, y in zip(*((c.k, c.v, c.k_scale, c.v_scale) for c in caches)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("inter,rot", [(False, 64), (True, 64), (False, 16), (True, 32), (False, 0), (False, 48)])
 def test_append_rotates_keys(acf, inter, rot):
     b = P.Batch(acf, [40, 1, 17], [100, 77, 17], 32, seed=6)
     cache = P.random_cache(acf, b.pages, 2, 64, 32, 7)
