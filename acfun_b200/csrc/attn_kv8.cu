@@ -28,7 +28,7 @@
 // asynchronously; nothing is shared between warps.
 //
 // Measured (B200): one fp16 token of 64 query heads over 262145 keys of 8 cache heads of 128 elements
-// 100 us, 5.4 TB/s, 82 % of the measured copy rate, at 1.65 GHz under the board's power limit; one
+// 101 us, 5.3 TB/s, 81 % of the measured copy rate, at 1.65 GHz under the board's power limit; one
 // token each of 48 sequences of 33 to 16000 keys, 32 query and 8 cache heads, 56 us, 4.0 TB/s, where
 // blocks that find no chunk of their own and the joins of short chunks cost the rest.
 #include <math.h>

@@ -24,7 +24,7 @@
 // between its weights and its next scores.
 //
 // Measured (B200, 32 query and 8 cache heads of 128 elements, bf16, causal): a prompt of 8192 tokens
-// 535 us, 1.03 PFLOP/s of what the mask leaves, 63 % of the measured bf16 peak, at 1.65 GHz under the
+// 539 us, 1.02 PFLOP/s of what the mask leaves, 62 % of the measured bf16 peak, at 1.65 GHz under the
 // board's power limit.  A step of 64 keys of both tiles takes about 1650 cycles; its products need
 // 1280, its 2^x 770 of the special function units (a quarter of them on the FMA units: none 1.22 and
 // half 1.11 times as long per softmax), and it issues 880 instructions per scheduler.  Two threads per

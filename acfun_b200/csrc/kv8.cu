@@ -9,10 +9,10 @@
 // are read once; the next head's are requested meanwhile.  1 / s is rounded once and multiplied by, as
 // the definition says, not divided by: a tie may fall to the other side of it, by half a code.
 //
-// Measured (B200, bf16, 8 heads of 128): append of 65551 tokens with rotation 136 us, 3.0 TB/s of what
-// it has to move: bound by instructions (20 per value; a page of 128 tokens takes a block of 1024
-// threads, whose barrier per head shows).  Read of 24 prefixes of 500 to 8191 tokens 83 us, 6.0 TB/s,
-// 92 % of the measured copy rate.
+// Measured (B200, bf16, 8 heads of 128): append of 65551 tokens with rotation 105 us, 3.8 TB/s of what
+// it has to move, 59 % of the measured copy rate: bound by instructions (18 per value; a page of 128
+// tokens takes a block of 1024 threads, whose barrier per head shows).  Read of 24 prefixes of 500 to
+// 8191 tokens 84 us, 6.0 TB/s, 92 % of the measured copy rate.
 #include <algorithm>
 
 #include "attn.cuh"
