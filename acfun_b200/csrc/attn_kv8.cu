@@ -576,14 +576,14 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
   if (p.a.beside) dev::grid_dep_wait();
 }
 
-// Zeroed once per device; the kernel leaves it zero.
-unsigned* tickets_of(int device) {
+// Zeroed once per device, in the stream of the call that needs it first (a call on another stream waits
+// for the calls before it, as for their scratch); the kernel leaves it zero.
+unsigned* tickets_of(Call& c, int device) {
   static unsigned* buf[64] = {};
-  if (device < 0 || device >= 64) return nullptr;
   if (!buf[device]) {
     unsigned* d = nullptr;
     if (!ACF_CUDA_OK(cudaMalloc(&d, kTickets * sizeof(unsigned)))) return nullptr;
-    if (!ACF_CUDA_OK(cudaMemset(d, 0, kTickets * sizeof(unsigned)))) {
+    if (!ACF_CUDA_OK(cudaMemsetAsync(d, 0, kTickets * sizeof(unsigned), c.stream()))) {
       cudaFree(d);
       return nullptr;
     }
@@ -638,7 +638,7 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
     p.part_ml = (float2*)c.scratch(n * sizeof(float2));
     if (work <= kTickets) {
-      p.tickets = tickets_of(current_device());
+      p.tickets = tickets_of(c, dv);
     } else {
       p.tickets = (unsigned*)c.scratch((size_t)work * sizeof(unsigned));
       if (p.tickets && !ACF_CUDA_OK(cudaMemsetAsync(p.tickets, 0, (size_t)work * sizeof(unsigned), c.stream())))

@@ -72,7 +72,6 @@ struct TcArgs {
   int splits;
   float* part_o;   // [tokens][q_heads][splits][DIM], null when splits == 1
   float2* part_ml;
-  int row_tiles;
   // images of the key tiles made before the kernel: [seqs][heads][tiles] of K, V and their scales
   uint8_t* k_img;
   uint8_t* v_img;
@@ -262,6 +261,64 @@ __global__ void __launch_bounds__(256) k_kv8_tiles(const TcArgs p, unsigned* err
   }
 }
 
+// Row tile `slot` of the batch's sequences in their order, the last rows of a sequence first (when causal
+// they see the most keys); seq is -1 past the end.  The host does not know the lengths: a grid of
+// [seqs][row tiles of max_new] left most blocks of a ragged batch without rows, and as a block takes an
+// SM, the full ones came late (11 sequences of 2 to 1300 tokens: SLOT_BEFORE us; so: SLOT_AFTER).  Each warp
+// scans the starts, 128 sequences at a time.
+struct Slot {
+  int seq, rt;
+  SeqView sv;
+};
+__device__ __forceinline__ Slot find_slot(const AttnArgs& a, int slot, unsigned* err) {
+  constexpr int K = 4;  // sequences per lane
+  const int lane = threadIdx.x & 31;
+  Slot s = {-1, 0, {0, 0, 0}};
+  for (int s0 = 0; s0 < a.b.seqs; s0 += 32 * K) {
+    SeqView v[K];
+    int tiles[K], mine = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = s0 + lane * K + k;
+      tiles[k] = 0;
+      if (i < a.b.seqs) {
+        v[k] = seq_view(a.b, i, err);
+        const int rows = v[k].n * a.group;
+        if (rows_taken(a, rows)) tiles[k] = (rows + kRows - 1) / kRows;
+      }
+      mine += tiles[k];
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, slot < upto);
+    if (past) {
+      const int owner = __ffs(past) - 1;
+      int left = slot - (upto - mine);
+      bool found = false;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (!found && left < tiles[k]) {
+          found = true;
+          s.seq = s0 + lane * K + k, s.rt = tiles[k] - 1 - left, s.sv = v[k];
+        }
+        left -= tiles[k];
+      }
+      s.seq = __shfl_sync(0xffffffffu, s.seq, owner);
+      s.rt = __shfl_sync(0xffffffffu, s.rt, owner);
+      s.sv.row0 = __shfl_sync(0xffffffffu, s.sv.row0, owner);
+      s.sv.n = __shfl_sync(0xffffffffu, s.sv.n, owner);
+      s.sv.len = __shfl_sync(0xffffffffu, s.sv.len, owner);
+      return s;
+    }
+    slot -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return s;
+}
+
 template <typename T, int DIM, bool PRE>
 __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArgs p, unsigned* err) {
   using L = TcSmem<DIM>;
@@ -274,12 +331,12 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
   float4* scales = reinterpret_cast<float4*>(smem + L::kScales);  // [ring][unit]: k factor, log2 v, 1 / v
   const AttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // late row tiles see the most keys when causal: they go first
-  const int head = blockIdx.x % a.kv.heads, rt = p.row_tiles - 1 - blockIdx.x / a.kv.heads;
-  const int seq = blockIdx.y, part = blockIdx.z;
-  const SeqView sv = seq_view(a.b, seq, err);
-  const int rows = sv.n * a.group, r0 = rt * kRows;
-  if (r0 >= rows || !rows_taken(a, rows)) return;
+  const int head = blockIdx.x % a.kv.heads, part = blockIdx.y;
+  const Slot slot = find_slot(a, blockIdx.x / a.kv.heads, err);
+  const int seq = slot.seq;
+  if (seq < 0) return;
+  const SeqView sv = slot.sv;
+  const int rows = sv.n * a.group, r0 = slot.rt * kRows;
   const int nr = min(kRows, rows - r0);
   const KeyRange kr = key_range(a, sv, r0, nr, kKeys);
   const int nsplit = max(1, (kr.n + p.chunk - 1) / p.chunk);
@@ -803,12 +860,18 @@ bool tc_run(Call& c, const AttnArgs& a, bool* last_is_main) {
   TcArgs p = {};
   p.a = a;
   const long long max_new = std::min(a.b.max_new, a.b.tokens);
-  p.row_tiles = (int)((max_new * a.group + kRows - 1) / kRows);
+  const long long row_tiles = (max_new * a.group + kRows - 1) / kRows;  // of one sequence
+  const long long slots = std::min(row_tiles * a.b.seqs, (long long)a.b.tokens * a.group / kRows + a.b.seqs);
+  const long long work = slots * a.kv.heads;
+  if (work > 0x7fffffffLL) {
+    set_error(kInvalid, "acfun_kv8_attention: too many rows");
+    return false;
+  }
   // few blocks: the keys are split so that every SM gets one, in parts of at least 4 key tiles
-  const long long work = (long long)p.row_tiles * a.kv.heads * a.b.seqs;
   const int tiles = (a.b.max_len + kKeys - 1) / kKeys;
   const long long want = std::max<long long>(1, c.sm_count() / std::max<long long>(1, work));
-  const int most = tiles + (a.window > 0);  // a window can start inside a tile
+  // most key tiles that a block's rows see; a window's can start and end inside a tile
+  const int most = a.window > 0 ? (int)std::min<long long>(tiles, ((long long)a.window + kRows / a.group + 1) / kKeys + 2) : tiles;
   p.chunk = (int)std::max<long long>(4, (most + want - 1) / want);
   p.splits = (most + p.chunk - 1) / p.chunk;
   if (p.splits > 1) {
@@ -819,8 +882,8 @@ bool tc_run(Call& c, const AttnArgs& a, bool* last_is_main) {
   }
   // tile images before the kernel: where the conversion would be repeated, and they fit
   const size_t images = (size_t)a.b.seqs * a.kv.heads * tiles;
-  const bool pre = p.row_tiles >= kPreRowTiles && images * (2 * kKeys * DIM * 2) <= kPreBytes;
-  const dim3 grid(p.row_tiles * a.kv.heads, a.b.seqs, p.splits);
+  const bool pre = row_tiles >= kPreRowTiles && images * (2 * kKeys * DIM * 2) <= kPreBytes;
+  const dim3 grid((unsigned)work, p.splits);
   if (pre) {
     p.tiles = tiles;
     p.k_img = (uint8_t*)c.scratch(images * kKeys * DIM * 2);
