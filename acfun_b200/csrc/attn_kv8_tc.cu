@@ -648,8 +648,10 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
       arrive(&bar.q_full);
     }
     const int pos = sv.len - sv.n + tok;
-    const int see_hi = !in || pos < 0 ? 0 : a.causal ? min(sv.len, pos + 1) : sv.len;
-    const int see_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    // a thread without a row masks nothing (its zeros of Q give results that are not written): the
+    // masking of a ragged end's warps made its block a quarter longer
+    const int see_hi = !in ? 0x7fffffff : pos < 0 ? 0 : a.causal ? min(sv.len, pos + 1) : sv.len;
+    const int see_lo = in && a.window > 0 ? max(0, pos - a.window + 1) : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
