@@ -323,8 +323,9 @@ template <typename T, int DIM, bool PRE>
 __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArgs p, unsigned* err) {
   using L = TcSmem<DIM>;
   extern __shared__ uint8_t smem_raw[];
-  // Launched normally: everything before it in the stream is complete.  Once every block has started,
-  // the streaming kernel of the same call may run on the SMs that are free.
+  // Once every block is past the wait, everything before this kernel in the stream is complete, and the
+  // streaming kernel of the same call may run on the SMs that are free.
+  dev::grid_dep_wait();
   dev::grid_dep_launch();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcBars& bar = *reinterpret_cast<TcBars*>(smem + L::kBars);
@@ -817,6 +818,8 @@ __global__ void __launch_bounds__(128) k_attn_join(const TcArgs p, unsigned* err
   const AttnArgs& a = p.a;
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, seq = blockIdx.y;
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
   const SeqView sv = seq_view(a.b, seq, err);
   if (item >= (long long)sv.n * a.q_heads || !rows_taken(a, sv.n * a.group)) return;
   const int tok = (int)(item / a.q_heads), hq = (int)(item - (long long)tok * a.q_heads);
@@ -853,7 +856,7 @@ bool tc_launch(Call& c, TcArgs p, dim3 grid) {
       return false;
     attr_done[dv] = true;
   }
-  k_attn_tc<T, DIM, PRE><<<grid, Roles<PRE>::kThreads, L::kBytes, c.stream()>>>(p, c.err());
+  if (!ACF_CUDA_OK(launch_pdl(k_attn_tc<T, DIM, PRE>, grid, dim3(Roles<PRE>::kThreads), (size_t)L::kBytes, c.stream(), p, c.err()))) return false;
   return c.launched("k_attn_tc");
 }
 
@@ -900,7 +903,8 @@ bool tc_run(Call& c, const AttnArgs& a, bool* last_is_main) {
   *last_is_main = p.splits == 1;
   if (p.splits > 1) {
     const long long items = (max_new * a.q_heads + 3) / 4;
-    k_attn_join<T, DIM><<<dim3((unsigned)items, a.b.seqs), 128, 0, c.stream()>>>(p, c.err());
+    const dim3 each((unsigned)items, a.b.seqs);
+    if (!ACF_CUDA_OK(launch_pdl(k_attn_join<T, DIM>, each, dim3(128), (size_t)0, c.stream(), p, c.err()))) return false;
     return c.launched("k_attn_join");
   }
   return true;
