@@ -313,6 +313,34 @@ def test_attention_decode_steps_beside_prompts(acf, dtype, hq, heads, dim):
     P.check_attention(got, lse, P.attention64(cache, b, q, dim ** -0.5, True, 0), dtype)
 
 
+@pytest.mark.parametrize("hq,heads,most", [(4, 1, 70), (3, 1, 300), (40, 1, 9)])
+def test_attention_of_many_ragged_sequences(acf, hq, heads, most):
+    """300 sequences, of which many have no new token and many few: row tiles are found by counting."""
+    rng = np.random.default_rng(most)
+    new = [int(x) for x in rng.integers(0, most + 1, 300) * (rng.random(300) < 0.6)]
+    new[0], new[127], new[128], new[299] = 0, most, most, most
+    b = P.Batch(acf, new, [n + int(x) for n, x in zip(new, rng.integers(0, 90, 300))], 16, seed=32)
+    cache = P.random_cache(acf, b.pages, heads, 64, 16, 33)
+    q = (randn(34, b.tokens, hq, 64) * 0.3).to(torch.float16)
+    got = cache.attention(q, b.h)
+    acf.synchronize()
+    P.check_attention(got, None, P.attention64(cache, b, q, 64 ** -0.5, True, 0), "f16")
+
+
+@pytest.mark.parametrize("dtype,dim,window,new,length", [
+    ("f16", 64, 700, [260], [3000]), ("bf16", 128, 1023, [87, 1], [4096, 900]), ("f16", 128, 1 << 30, [60], [2000]),
+    ("bf16", 64, 513, [333], [333]), ("f16", 64, 1, [100], [5000])])
+def test_attention_windows_in_parts(acf, dtype, dim, window, new, length):
+    """Few row tiles, whose windows are divided among blocks."""
+    b = P.Batch(acf, new, length, 32, seed=35)
+    cache = P.random_cache(acf, b.pages, 2, dim, 32, 36)
+    q = (randn(37, b.tokens, 6, dim) * 0.3).to(P.DT[dtype])
+    lse = torch.full((b.tokens, 6), 7.0, device="cuda")
+    got = cache.attention(q, b.h, window=window, lse=lse)
+    acf.synchronize()
+    P.check_attention(got, lse, P.attention64(cache, b, q, dim ** -0.5, True, window), dtype)
+
+
 def test_attention_of_very_many_sequences(acf):
     """More (sequence, head) pairs than the standing tickets, one of them split by the bound on a
     chunk's pages."""
