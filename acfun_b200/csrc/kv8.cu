@@ -405,13 +405,15 @@ bool append_run(Call& c, AppendArgs a) {
   parts = (a.kv.heads + a.head_block - 1) / a.head_block;
   const int threads = per_head * std::max(1, std::min(a.head_block, 256 / per_head));
   const size_t smem = (size_t)std::min(page, a.b.max_new) * (a.rot / 2) * sizeof(float2);
+  // The most that any call takes is asked for at the first one: 48 KiB hold without asking, but for the
+  // static arrays too.
   static bool attr_done[64] = {false};
-  const int dv = current_device();
-  if (smem > 48 * 1024 && !attr_done[dv & 63]) {
+  const int dv = current_device() & 63;
+  if (!attr_done[dv]) {
     if (!ACF_CUDA_OK(cudaFuncSetAttribute(k_kv8_append<T, DIM, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           128 * (DIM / 2) * (int)sizeof(float2))))
       return false;
-    attr_done[dv & 63] = true;
+    attr_done[dv] = true;
   }
   if (!ACF_CUDA_OK(launch_pdl(k_kv8_append<T, DIM, VEC>, dim3(slots, 2 * parts, a.b.seqs), dim3(threads), smem, c.stream(), a,
                               c.err())))
