@@ -31,6 +31,7 @@ void clear_error();
   ([&]() -> bool {                                                                         \
     cudaError_t e__ = (expr);                                                              \
     if (e__ != cudaSuccess) {                                                              \
+      cudaGetLastError(); /* reported here, not by the next launch check */                \
       ::acf::set_error(e__ == cudaErrorMemoryAllocation ? ::acf::kNoMem : ::acf::kCuda,   \
                        "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e__), __FILE__, \
                        __LINE__);                                                          \
