@@ -719,7 +719,9 @@ extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatc
   if (!c.ok()) return last_error_code();
   a.q_token = q_token, a.q_head = q_head, a.o_token = o_token, a.o_head = o_head;
   a.dtype = dtype, a.q_heads = q_heads, a.group = q_heads / cache->heads;
-  a.scale = scale, a.causal = causal != 0, a.window = window;
+  a.scale = scale, a.causal = causal != 0;
+  // a window that holds any sequence hides nothing (and in the kernels position - window stays in range)
+  a.window = window < batch->max_len ? window : 0;
   // Sequences with more than 32 rows per cache head go to the tensor cores' tiles of 128, the others are
   // streamed.  Measured with 32 query and 8 cache heads of 128 elements, 16 sequences of 4096 keys:
   // 16 rows 56 us streamed and 88 us tiled, 32 rows 80 and 84, 64 rows 132 and 85.  A batch may hold
