@@ -215,10 +215,10 @@ class KvCache8:
     def read(self, batch: KvBatch, dtype):
         """(k, v) [tokens, heads, dim]: the last start[i + 1] - start[i] tokens of each sequence."""
         code = _dtype_code(dtype)
-        like = batch.likes.get((dtype, self.heads, self.dim))
+        key = dtype, self.heads, self.dim, self.k.device
+        like = batch.likes.get(key)
         if like is None:  # one element that has the outputs' shape: making them like it is the shortest call
-            like = self.k.new_empty(1, dtype=dtype).expand(batch.tokens, self.heads, self.dim)
-            batch.likes[dtype, self.heads, self.dim] = like
+            like = batch.likes[key] = self.k.new_empty(1, dtype=dtype).expand(batch.tokens, self.heads, self.dim)
         global _empty_like
         if _empty_like is None:
             from torch import empty_like as _empty_like

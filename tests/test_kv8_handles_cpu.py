@@ -1,0 +1,33 @@
+"""CPU: what the Python handles of the int8 cache keep and pass on, with the library's calls replaced."""
+import numpy as np
+import pytest
+import torch
+
+import acfun_b200 as acf
+from acfun_b200 import kv8
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Name -> arguments of the last call, which does nothing and succeeds."""
+    seen = {}
+    for name in ("acfun_rope", "acfun_kv8_append", "acfun_kv8_read", "acfun_kv8_attention"):
+        monkeypatch.setitem(kv8._calls, name, lambda *a, name=name: seen.update({name: a}) and 0)
+    return seen
+
+
+def batch(tokens=3, max_new=3, max_len=9):
+    return acf.KvBatch(np.zeros((1, 1), np.int32), np.array([0, tokens], np.int32), np.array([max_len], np.int32), tokens, max_new, max_len)
+
+
+def test_one_batch_for_caches_on_two_devices(calls):
+    """Index arrays may be host memory, so one batch can serve the layers of several devices: what is read
+    is on the device of the cache it was read from."""
+    b = batch()
+    for _ in range(2):
+        for device in ("cpu", "meta"):
+            for heads, dim in ((2, 64), (2, 128)):
+                cache = acf.KvCache8.empty(1, heads, dim, 16, device=device)
+                for dtype in (torch.float16, torch.float32):
+                    for x in cache.read(b, dtype):
+                        assert x.device.type == device and x.dtype == dtype and x.shape == (3, heads, dim) and x.is_contiguous()
