@@ -645,6 +645,35 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
           *reinterpret_cast<uint4*>(p16) = o;
         }
       }
+      // Where K takes bf16 as q does, a row's products with codes can pass 2^128 although its scores do not:
+      // such a row is brought down by a power of two, in place and exactly, and so is one so small that
+      // its products would be subnormal brought up.
+      if constexpr (PRE && std::is_same<T, __nv_bfloat16>::value) {
+        __syncwarp();
+        uint8_t* mine = tile + row * 128;
+        auto part = [&](int k) { return reinterpret_cast<uint4*>(mine + (k >> 3) * (128 * 128) + (((k & 7) ^ (row & 7)) << 4)); };
+        __nv_bfloat162 most = __float2bfloat162_rn(0.0f);
+#pragma unroll 4
+        for (int k = 0; k < DIM / 8; ++k) {
+          const uint4 w = *part(k);
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = __hmax2(most, __habs2(x[e]));
+        }
+        const float top = fmaxf(__low2float(most), __high2float(most));
+        if (top > 0x1p40f || (top > 0.0f && top < 0x1p-40f)) {
+          const Pow2 f = row_pow2(top);
+          q_unit = f.up;
+#pragma unroll 1
+          for (int k = 0; k < DIM / 8; ++k) {
+            float x[8];
+            load8(reinterpret_cast<const T*>(part(k)), true, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= f.down;
+            store8(reinterpret_cast<T*>(part(k)), true, x);
+          }
+        }
+      }
       dev::fence_proxy_async_smem();
       arrive(&bar.q_full);
     }
@@ -657,83 +686,127 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     const bool active = t == 0 || two;
-    for (int i = 0; i < steps && active; ++i) {
-      const uint32_t tS = tS0 + t * 128 + (i & 1) * kStep + lanes;
-      if (!(ok = wait(&bar.s_full[t][i & 1], (i >> 1) & 1))) break;
-      dev::tc_fence_after();
-      float s[kStep];
-      tmem_ld32p(tS, s);
-      tmem_ld32p(tS + 32, s + 32);
-      dev::tmem_ld_wait();
-      const float4* sc = scales + ((i >> 1) % kScaleRing) * kUnits + (i & 1) * (kUnits / 2);
-      const int k0 = tile0 * kKeys + i * kStep;
-      const int lo = see_lo - k0, hi = see_hi - k0;
-      if (__any_sync(0xffffffffu, lo > 0 || hi < kStep)) {
-        // opaque bounds: the comparisons stay inside this branch instead of running for every step
-        int from = lo, to = hi;
-        asm volatile("" : "+r"(from), "+r"(to));
+    // Rows that the common form of a weight does not serve (`odd`) go by their scores, formed in place of S
+    // before the maximum, and turned back after it into what that form makes the same weights of.  A
+    // warp with such a row takes a loop of its own: in the one loop this took 3 % of a long prompt (488
+    // against 473 us in a burst).
+    bool odd = PRE && q_unit != 1.0f;
+    auto factor = [&](const float4& f) { return fmaxf(PRE ? f.x : f.x * q_unit, kLeast); };
+    // Steps from i on; the first one that was not done.
+    auto softmax = [&](int i, auto with_odd) -> int {
+      constexpr bool ODD = decltype(with_odd)::value;
+      for (; i < steps; ++i) {
+        const uint32_t tS = tS0 + t * 128 + (i & 1) * kStep + lanes;
+        if (!(ok = wait(&bar.s_full[t][i & 1], (i >> 1) & 1))) return i;
+        dev::tc_fence_after();
+        float s[kStep];
+        tmem_ld32p(tS, s);
+        tmem_ld32p(tS + 32, s + 32);
+        dev::tmem_ld_wait();
+        const float4* sc = scales + ((i >> 1) % kScaleRing) * kUnits + (i & 1) * (kUnits / 2);
+        const int k0 = tile0 * kKeys + i * kStep;
+        const int lo = see_lo - k0, hi = see_hi - k0;
+        if (__any_sync(0xffffffffu, lo > 0 || hi < kStep)) {
+          // opaque bounds: the comparisons stay inside this branch instead of running for every step
+          int from = lo, to = hi;
+          asm volatile("" : "+r"(from), "+r"(to));
 #pragma unroll
-        for (int e = 0; e < kStep; ++e)
-          if (e < from || e >= to) s[e] = -INFINITY;
-      }
-      float top = -INFINITY;
+          for (int e = 0; e < kStep; ++e)
+            if (e < from || e >= to) s[e] = -INFINITY;
+        }
+        float top = -INFINITY;
+        auto scores = [&] {
+          top = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < kStep / 16; ++u) {
-        const float* v = s + 16 * u;
-        const float x0 = max3(max3(v[0], v[1], v[2]), v[3], v[4]), x1 = max3(max3(v[5], v[6], v[7]), v[8], v[9]);
-        const float x2 = max3(max3(v[10], v[11], v[12]), v[13], v[14]);
-        const float4 f = sc[u];
-        top = fmaxf(top, fmaf(max3(fmaxf(x0, v[15]), x1, x2), fmaxf(f.x * q_unit, kLeast), f.y));
-      }
-      if (__any_sync(0xffffffffu, top > m + kMost)) {
-        const float n = fmaxf(m, top - kTop);
-        const float b = m == n ? 1.0f : ex2(m - n);
-        m = n;
-        l *= b;
-        if (i > 0) {  // O holds the steps before this one, once the last of them is done
-          if (!(ok = wait(&bar.o_step[t], (i - 1) & 1))) break;
-          dev::tc_fence_after();
+          for (int u = 0; u < kStep / 16; ++u) {
+            const float4 f = sc[u];
+            const float fx = fmaxf(f.x * q_unit, kLeast);
+#pragma unroll
+            for (int e = 16 * u; e < 16 * u + 16; ++e) s[e] = fmaf(s[e], fx, f.y), top = fmaxf(top, s[e]);
+          }
+        };
+        if (ODD && odd) {
+          scores();
+        } else {
+#pragma unroll
+          for (int u = 0; u < kStep / 16; ++u) {
+            const float* v = s + 16 * u;
+            const float x0 = max3(max3(v[0], v[1], v[2]), v[3], v[4]), x1 = max3(max3(v[5], v[6], v[7]), v[8], v[9]);
+            const float x2 = max3(max3(v[10], v[11], v[12]), v[13], v[14]);
+            const float4 f = sc[u];
+            top = fmaxf(top, fmaf(max3(fmaxf(x0, v[15]), x1, x2), factor(f), f.y));
+          }
+        }
+        if (__any_sync(0xffffffffu, top > m + kMost)) {
+          const float n = fmaxf(m, top - kTop);
+          const float b = m == n ? 1.0f : ex2(m - n);
+          m = n;
+          l *= b;
+          if (i > 0) {  // O holds the steps before this one, once the last of them is done
+            if (!(ok = wait(&bar.o_step[t], (i - 1) & 1))) return i;
+            dev::tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < DIM / 16; ++c) {
-            float o[16];
-            tmem_ld16p(tO0 + t * DIM + lanes + c * 16, o);
-            dev::tmem_ld_wait();
-            uint32_t x[16];
+            for (int c = 0; c < DIM / 16; ++c) {
+              float o[16];
+              tmem_ld16p(tO0 + t * DIM + lanes + c * 16, o);
+              dev::tmem_ld_wait();
+              uint32_t x[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * b);
-            tmem_st16(tO0 + t * DIM + lanes + c * 16, x);
-          }
-        }
-      }
-      const float m0 = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int h = 0; h < kStep / 32; ++h) {  // 32 keys: 16 registers of weights
-        uint32_t w[16];
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const int u = 2 * h + v;
-          const float4 f = sc[u];
-          const float fx = fmaxf(f.x * q_unit, kLeast), off = f.y - m0;
-          const float2 fx2 = make_float2(fx, fx), off2 = make_float2(off, off);
-          float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float2 x = fma2(make_float2(s[16 * u + e], s[16 * u + e + 1]), fx2, off2);
-            if ((e / 2) % 4 >= kFmaOf4) {
-              x.x = ex2(x.x), x.y = ex2(x.y);
-            } else {
-              x = ex2_fma2(x);
+              for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * b);
+              tmem_st16(tO0 + t * DIM + lanes + c * 16, x);
             }
-            sum = add2(sum, x);
-            w[8 * v + e / 2] = pack_f16(x.x, x.y);
           }
-          l = fmaf(sum.x + sum.y, f.z, l);
         }
-        tmem_st16(tS + 16 * h, w);
+        float m0 = m == -INFINITY ? 0.0f : m;
+        if constexpr (ODD) {
+          if (odd) {  // s * factor + (f.y - 0) is to be score - m0
+#pragma unroll
+            for (int u = 0; u < kStep / 16; ++u) {
+              const float4 f = sc[u];
+              const float r = 1.0f / factor(f);
+#pragma unroll
+              for (int e = 16 * u; e < 16 * u + 16; ++e) s[e] = s[e] == -INFINITY ? s[e] : ((s[e] - m0) - f.y) * r;
+            }
+            m0 = 0.0f;
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < kStep / 32; ++h) {  // 32 keys: 16 registers of weights
+          uint32_t w[16];
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const int u = 2 * h + v;
+            const float4 f = sc[u];
+            const float fx = factor(f), off = f.y - m0;
+            const float2 fx2 = make_float2(fx, fx), off2 = make_float2(off, off);
+            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float2 x = fma2(make_float2(s[16 * u + e], s[16 * u + e + 1]), fx2, off2);
+              if ((e / 2) % 4 >= kFmaOf4) {
+                x.x = ex2(x.x), x.y = ex2(x.y);
+              } else {
+                x = ex2_fma2(x);
+              }
+              sum = add2(sum, x);
+              w[8 * v + e / 2] = pack_f16(x.x, x.y);
+            }
+            l = fmaf(sum.x + sum.y, f.z, l);
+          }
+          tmem_st16(tS + 16 * h, w);
+        }
+        tmem_st_wait();
+        dev::tc_fence_before();
+        arrive(&bar.p_full[t][i & 1]);
       }
-      tmem_st_wait();
-      dev::tc_fence_before();
-      arrive(&bar.p_full[t][i & 1]);
+      return steps;
+    };
+    if (active) {
+      if (PRE && std::is_same<T, __nv_bfloat16>::value && __any_sync(0xffffffffu, odd))
+        softmax(0, std::true_type());
+      else
+        softmax(0, std::false_type());
     }
     if (ok && ntiles > 0) ok = wait(&bar.o_full, 0);
     dev::tc_fence_after();
