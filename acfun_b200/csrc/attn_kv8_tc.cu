@@ -59,6 +59,10 @@ constexpr int kStep = 64;      // keys of one S product and its softmax
 constexpr int kUnits = kKeys / 16;
 constexpr int kFmaOf4 = 1;      // pairs of four whose 2^x the FMA units compute instead of the special function unit
 constexpr float kLeast = 1e-37f;  // a factor never underflows to 0: a masked score stays -inf under it
+// The offset from which a row's weights are taken from its rounded scores.  The common form, one fused
+// operation on S, sees the rounding of the offset: below this within 2 powers of two, which kTop leaves
+// room for, but from 2^27 on past fp16.
+constexpr float kFar = 0x1p24f;
 // Row tiles from which the key tiles are converted before the kernel (32 query, 8 cache heads of 128:
 // 16 row tiles 34.5 us converted in the kernel and 35.0 us before it, 32 row tiles 60.6 and 55.5), and
 // the most scratch that this may take.
@@ -686,10 +690,11 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     const bool active = t == 0 || two;
-    // Rows that the common form of a weight does not serve (`odd`) go by their scores, formed in place of S
-    // before the maximum, and turned back after it into what that form makes the same weights of.  A
-    // warp with such a row takes a loop of its own: in the one loop this took 3 % of a long prompt (488
-    // against 473 us in a burst).
+    // Rows that the common form of a weight does not serve (`odd`: those with a factor of their own beside K
+    // in bf16, and those whose offset has passed kFar) go by their scores, formed in place of S before the
+    // maximum, and turned back after it into what that form makes the same weights of.  A warp with such a
+    // row takes a loop of its own: in the one loop this took 3 % of a long prompt (488 against 473 us in a
+    // burst).
     bool odd = PRE && q_unit != 1.0f;
     auto factor = [&](const float4& f) { return fmaxf(PRE ? f.x : f.x * q_unit, kLeast); };
     // Steps from i on; the first one that was not done.
@@ -739,6 +744,12 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
         }
         if (__any_sync(0xffffffffu, top > m + kMost)) {
           const float n = fmaxf(m, top - kTop);
+          if constexpr (ODD) {
+            if (!odd && fabsf(n) >= kFar && n != -INFINITY) odd = true, scores();
+            __syncwarp();
+          } else {
+            if (__any_sync(0xffffffffu, fabsf(n) >= kFar && n != -INFINITY)) return i;  // again, in the other loop
+          }
           const float b = m == n ? 1.0f : ex2(m - n);
           m = n;
           l *= b;
@@ -803,10 +814,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1) k_attn_tc(const TcArg
       return steps;
     };
     if (active) {
-      if (PRE && std::is_same<T, __nv_bfloat16>::value && __any_sync(0xffffffffu, odd))
-        softmax(0, std::true_type());
-      else
-        softmax(0, std::false_type());
+      const int i = __any_sync(0xffffffffu, odd) ? 0 : softmax(0, std::false_type());
+      if (ok && i < steps) softmax(i, std::true_type());
     }
     if (ok && ntiles > 0) ok = wait(&bar.o_full, 0);
     dev::tc_fence_after();
