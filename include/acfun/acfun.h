@@ -170,8 +170,9 @@ int acfun_set_fp32_math(int mode);
  * token and head strides in elements (dim is contiguous), so a slice of a packed q/k/v row can
  * be passed in place.  All functions return 0 or an error code (also in acfun_last_error()) and
  * check their arguments on the host; entries of device arrays (table, start, length) are checked
- * in the kernels: a bad one skips its sequence and is reported, as code 1, by the next
- * acfun_synchronize().  Activations and index arrays may be host memory; the cache itself must be
+ * in the kernels: a bad one skips its sequence (a bad offset those on both sides of it; where offsets
+ * decrease, rows of other sequences may be left as they are too) and is reported, as code 1, by the
+ * next acfun_synchronize().  Activations and index arrays may be host memory; the cache itself must be
  * device memory. */
 #define ACFUN_F32 0
 #define ACFUN_F16 1
