@@ -174,7 +174,7 @@ extern "C" int acfun_rope_frequencies(int rot, double base, int scaling, double 
   if (rot <= 0 || rot % 2) bad = "rot must be positive and even";
   else if (!(base > 1.0) || !isfinite(base)) bad = "base must be above 1";
   else if (!freq) bad = "freq is NULL";
-  else if (scaling < 0 || scaling > 4) bad = "scaling must be 0 to 4";
+  else if (scaling < 0 || scaling > 5) bad = "scaling must be 0 to 5";
   else if (scaling && (!(factor >= 1.0) || !isfinite(factor))) bad = "factor must be at least 1";
   else if (scaling == 2 && rot < 4) bad = "scaling 2 needs rot of at least 4";
   else if (scaling >= 3 && (!(trained > 0.0) || !isfinite(trained) || !(slow > 0.0) || !(fast > slow) || !isfinite(fast)))
@@ -192,8 +192,12 @@ extern "C" int acfun_rope_frequencies(int rot, double base, int scaling, double 
     if (scaling == 1) f /= factor;
     if (scaling >= 3) {
       double keep;  // the share of the unscaled frequency
-      if (scaling == 3) {
-        const double lo = index_of(fast), hi = index_of(slow);
+      if (scaling != 4) {
+        double lo = index_of(fast), hi = index_of(slow);
+        if (scaling == 5) {
+          lo = fmax(floor(lo), 0.0), hi = fmin(ceil(hi), rot - 1.0);
+          if (hi <= lo) hi = lo + 1e-3;  // both ends past the last pair
+        }
         keep = (hi - i) / (hi - lo);
       } else {
         keep = (trained * f / tau - slow) / (fast - slow);
@@ -203,7 +207,7 @@ extern "C" int acfun_rope_frequencies(int rot, double base, int scaling, double 
     }
     freq[i] = (float)f;
   }
-  if (amplitude) *amplitude = scaling == 3 ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
+  if (amplitude) *amplitude = scaling == 3 || scaling == 5 ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
   return 0;
 }
 

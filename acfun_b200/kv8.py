@@ -126,10 +126,11 @@ class Rope:
 def rope_frequencies(rot, base=10000.0, scaling=None, factor=1.0, trained=0, fast=32.0, slow=1.0):
     """(freq, amplitude): numpy fp32 [rot / 2] and a float.  scaling: None; "linear" (positions
     divided by factor); "base" (base enlarged so that the lowest frequency is divided by factor);
-    "by_parts" or "by_turns" (frequencies kept, divided or mixed by how often a pair turns within the
-    `trained` length: above `fast` turns, below `slow`, between; mixed linearly in the pair's index
-    or in the turns)."""
-    kinds = {None: 0, "linear": 1, "base": 2, "by_parts": 3, "by_turns": 4}
+    "by_parts", "by_whole_parts" or "by_turns" (frequencies kept, divided or mixed by how often a pair
+    turns within the `trained` length: above `fast` turns, below `slow`, between; mixed linearly in the
+    pair's index, in it between ends rounded outward to whole pairs, as checkpoints of this scaling
+    commonly have it, or in the turns)."""
+    kinds = {None: 0, "linear": 1, "base": 2, "by_parts": 3, "by_turns": 4, "by_whole_parts": 5}
     if scaling not in kinds:
         raise ValueError(f"scaling {scaling!r} is not one of {sorted(k for k in kinds if k)}")
     if rot <= 0:

@@ -216,7 +216,9 @@ typedef struct AcfunRope {
  *   3  by wavelength: pairs that turn more than `fast` times in the trained length keep their
  *      frequency, those below `slow` turns are divided by factor, linear in the pair's index
  *      between; amplitude 0.1 ln(factor) + 1
- *   4  as 3, linear in the number of turns between, amplitude 1 */
+ *   4  as 3, linear in the number of turns between, amplitude 1
+ *   5  as 3 with the ends of the linear part rounded outward to whole pairs (and kept within [0,
+ *      rot - 1]): the form that checkpoints of this scaling are made with unless they say otherwise */
 int acfun_rope_frequencies(int rot, double base, int scaling, double factor, double trained,
                            double fast, double slow, float* freq, float* amplitude);
 /* y = x with positions pos[token] in [0, 2^31) applied; rot even and at most dim; y may be x. */
