@@ -73,6 +73,8 @@ def _rows(x, what):
     if len(shape) != 3:
         raise ValueError(f"{what} must be [tokens, heads, dim], got {tuple(shape)}")
     if isinstance(x, np.ndarray):
+        if any(s % x.itemsize for s in x.strides):
+            raise ValueError(f"{what}: strides {x.strides} are not whole elements of {x.itemsize} bytes")
         t, h, d = (s // x.itemsize for s in x.strides)
         at = x.ctypes.data
     else:

@@ -31,3 +31,17 @@ def test_one_batch_for_caches_on_two_devices(calls):
                 for dtype in (torch.float16, torch.float32):
                     for x in cache.read(b, dtype):
                         assert x.device.type == device and x.dtype == dtype and x.shape == (3, heads, dim) and x.is_contiguous()
+
+
+def test_byte_strides_that_are_not_whole_elements_are_refused(calls):
+    """Rows of a record array whose records end in an odd byte: no stride in elements says where they are."""
+    x = np.zeros(3, np.dtype([("x", np.float16, (2, 64)), ("flag", np.uint8)]))["x"]
+    even = np.zeros(3, np.dtype([("x", np.float16, (2, 64)), ("flag", np.uint16)]))["x"]
+    cache = acf.KvCache8.empty(1, 2, 64, 16, device="cpu")
+    spec, pos, b = acf.Rope(np.ones(32, np.float32)), np.zeros(3, np.int32), batch()
+    for call in (lambda v: acf.rope(v, pos, spec), lambda v: acf.rope(np.zeros((3, 2, 64), np.float16), pos, spec, out=v),
+                 lambda v: cache.append(v, even, b), lambda v: cache.append(even, v, b), lambda v: cache.attention(v, b)):
+        with pytest.raises(ValueError, match="stride"):
+            call(x)
+        call(even)
+    assert calls["acfun_rope"][6] == 2 * 64 and calls["acfun_kv8_attention"][6] == 2 * 64 + 1
