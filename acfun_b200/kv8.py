@@ -66,12 +66,25 @@ def _flat(x, code, what):
     return _address(x)
 
 
+_INT = 0x7fffffff
+
+
+def _int(x, what):
+    """x as a C int; ctypes would cut it to its low 32 bits."""
+    x = int(x)
+    if not -_INT <= x <= _INT:
+        raise ValueError(f"{what} {x} does not fit 32 bits")
+    return x
+
+
 def _rows(x, what):
     """(address, dtype code, shape, token stride, head stride) of [tokens, heads, dim]; strides in
     elements."""
     shape = x.shape
     if len(shape) != 3:
         raise ValueError(f"{what} must be [tokens, heads, dim], got {tuple(shape)}")
+    if shape[0] > _INT:
+        raise ValueError(f"{what}: {shape[0]} tokens do not fit 32 bits")
     if isinstance(x, np.ndarray):
         if any(s % x.itemsize for s in x.strides):
             raise ValueError(f"{what}: strides {x.strides} are not whole elements of {x.itemsize} bytes")
@@ -135,7 +148,7 @@ def rope_frequencies(rot, base=10000.0, scaling=None, factor=1.0, trained=0, fas
     kinds = {None: 0, "linear": 1, "base": 2, "by_parts": 3, "by_turns": 4, "by_whole_parts": 5}
     if scaling not in kinds:
         raise ValueError(f"scaling {scaling!r} is not one of {sorted(k for k in kinds if k)}")
-    if rot <= 0:
+    if _int(rot, "rot") <= 0:
         raise ValueError("rot must be positive")
     freq = np.empty(rot // 2, np.float32)
     amp = C.c_float()
@@ -169,10 +182,10 @@ class KvBatch:
             raise ValueError("table must be [seqs, columns], start [seqs + 1] and length [seqs]")
         self.arrays = (table, start, length)
         self.likes = {}
-        self.tokens = int(tokens)
+        self.tokens = _int(tokens, "tokens")
         self.c = _Batch(_flat(table, _I32, "table"), _flat(start, _I32, "start"),
-                        _flat(length, _I32, "length"), table.shape[0], table.shape[1], self.tokens, int(max_new),
-                        int(max_len))
+                        _flat(length, _I32, "length"), table.shape[0], table.shape[1], self.tokens,
+                        _int(max_new, "max_new"), _int(max_len, "max_len"))
         self.ref = C.byref(self.c)
 
 
@@ -239,6 +252,8 @@ class KvCache8:
             raise ValueError(f"q must be [{batch.tokens}, q_heads, {self.dim}], got {tuple(shape)}")
         if lse is not None and tuple(lse.shape) != tuple(shape[:2]):
             raise ValueError("lse must be [tokens, q_heads]")
+        if window and not 0 < window <= _INT:  # beyond: no limit, as the longest
+            window = _INT if window > 0 else -1
         out, out_at, ot, oh = _out(out, q, shape, code, "q")
         err = _fn("acfun_kv8_attention")(self.ref, batch.ref, at, out_at, code, shape[1], qt, qh, ot, oh,
                                          self.dim ** -0.5 if scale is None else scale, int(bool(causal)), window,

@@ -45,3 +45,19 @@ def test_byte_strides_that_are_not_whole_elements_are_refused(calls):
             call(x)
         call(even)
     assert calls["acfun_rope"][6] == 2 * 64 and calls["acfun_kv8_attention"][6] == 2 * 64 + 1
+
+
+def test_sizes_past_32_bits_are_not_cut(calls):
+    for sizes in (dict(tokens=2 ** 32 + 3), dict(max_new=2 ** 32 + 3), dict(max_len=2 ** 31), dict(max_len=-2 ** 32 + 9)):
+        with pytest.raises(ValueError, match="32 bits"):
+            acf.KvBatch(np.zeros((1, 1), np.int32), np.zeros(2, np.int32), np.zeros(1, np.int32), **dict(dict(tokens=3, max_new=3, max_len=9), **sizes))
+    cache = acf.KvCache8.empty(1, 2, 64, 16, device="cpu")
+    q = np.zeros((3, 2, 64), np.float16)
+    for window, passed in ((0, 0), (5, 5), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 32 + 5, 2 ** 31 - 1), (2 ** 63, 2 ** 31 - 1), (-1, -1), (-2 ** 32 + 5, -1)):
+        cache.attention(q, batch(), window=window)
+        assert calls["acfun_kv8_attention"][12] == passed
+    long = torch.zeros(1, dtype=torch.float16).expand(2 ** 32 + 1, 1, 8)
+    with pytest.raises(ValueError, match="32 bits"):
+        acf.rope(long, torch.zeros(1, dtype=torch.int32).expand(2 ** 32 + 1), acf.Rope(np.ones(4, np.float32)), out=long)
+    with pytest.raises(ValueError, match="32 bits"):
+        acf.rope_frequencies(2 ** 32 + 64)
