@@ -577,8 +577,8 @@ __global__ void __launch_bounds__(kWarps * 32, DIM * R8 >= 512 ? 2 : 3) k_attn_s
 }
 
 // Zeroed once per device, in the stream of the call that needs it first (a call on another stream waits
-// for the calls before it, as for their scratch); the kernel leaves it zero.
-unsigned* tickets_of(Call& c, int device) {
+// for the calls before it, as for their scratch); the kernel leaves it zero.  *zeroed: by this call.
+unsigned* tickets_of(Call& c, int device, bool* zeroed) {
   static unsigned* buf[64] = {};
   if (!buf[device]) {
     unsigned* d = nullptr;
@@ -588,6 +588,7 @@ unsigned* tickets_of(Call& c, int device) {
       return nullptr;
     }
     buf[device] = d;
+    *zeroed = true;
   }
   return buf[device];
 }
@@ -637,13 +638,16 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     const size_t n = (size_t)a.b.seqs * a.kv.heads * p.part_rows * p.splits;
     p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
     p.part_ml = (float2*)c.scratch(n * sizeof(float2));
+    bool zeroed = false;
     if (work <= kTickets) {
-      p.tickets = tickets_of(c, dv);
+      p.tickets = tickets_of(c, dv, &zeroed);
     } else {
       p.tickets = (unsigned*)c.scratch((size_t)work * sizeof(unsigned));
       if (p.tickets && !ACF_CUDA_OK(cudaMemsetAsync(p.tickets, 0, (size_t)work * sizeof(unsigned), c.stream())))
         return false;
+      zeroed = true;
     }
+    if (zeroed) p.a.beside = false;  // the operation before in the stream is the memset, and is waited for
     if (!c.ok() || !p.tickets) return false;
   }
   const int smem = kBase + (int)std::min<long long>(chunk / a.kv.page + 2, kMaxPages) * (int)sizeof(PageEntry);
