@@ -639,7 +639,7 @@ bool stream_launch(Call& c, const AttnArgs& a) {
     p.part_o = (float*)c.scratch(n * DIM * sizeof(float));
     p.part_ml = (float2*)c.scratch(n * sizeof(float2));
     bool zeroed = false;
-    if (work <= kTickets) {
+    if (work <= kTickets && !c.capturing()) {
       p.tickets = tickets_of(c, dv, &zeroed);
     } else {
       p.tickets = (unsigned*)c.scratch((size_t)work * sizeof(unsigned));
@@ -712,7 +712,7 @@ extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatc
     set_error(kInvalid, "%s: q or out is NULL", what);
     return kInvalid;
   }
-  Call c(what);
+  Call c(what, true);
   if (!c.ok()) return last_error_code();
   AttnArgs a = {};
   a.kv = cache_view(cache);

@@ -566,7 +566,7 @@ extern "C" int acfun_kv8_append(const AcfunKvCache8* cache, const AcfunKvBatch* 
     set_error(kInvalid, "%s: k or v is NULL", what);
     return kInvalid;
   }
-  Call c(what);
+  Call c(what, true);
   if (!c.ok()) return last_error_code();
   AppendArgs a = {};
   a.kv = cache_view(cache);
@@ -592,7 +592,7 @@ extern "C" int acfun_kv8_read(const AcfunKvCache8* cache, const AcfunKvBatch* ba
   if (int e = check_cache(what, cache)) return e;
   if (int e = check_batch(what, batch, cache->page)) return e;
   if (batch->seqs == 0 || batch->tokens == 0 || batch->max_new == 0 || (!k && !v)) return 0;
-  Call c(what);
+  Call c(what, true);
   if (!c.ok()) return last_error_code();
   ReadArgs a = {};
   a.kv = cache_view(cache);

@@ -236,7 +236,7 @@ extern "C" int acfun_rope(const void* x, void* y, int dtype, int tokens, int hea
     set_error(kInvalid, "%s: in place needs equal strides", what);
     return kInvalid;
   }
-  Call c(what);
+  Call c(what, true);
   if (!c.ok()) return last_error_code();
   RopeArgs a = {};
   const size_t yb = span_bytes(y_token, y_head, tokens, heads, dim, dtype);

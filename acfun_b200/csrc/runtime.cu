@@ -153,13 +153,18 @@ bool check_device_error(DeviceState* d, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------------ Call
-Call::Call(const char* name) : name_(name) {
+Call::Call(const char* name, bool capturable) : name_(name), capturable_(capturable) {
   ThreadCtx& t = tctx();
   dev_ = device_state();
   if (!dev_) return;
   if (!ACF_CUDA_OK(cudaSetDevice(t.device))) return;
   lock_ = std::unique_lock<std::mutex>(dev_->mu);
   stream_ = t.stream;
+  // under capture neither may be synchronised with or freed, and nothing of the workspace is used
+  if ((dev_->ws_stream != stream_ || dev_->ws.in_parts()) && capturing()) {
+    ok_ = true;
+    return;
+  }
   if (dev_->ws_stream != stream_) {
     // scratch may still be in use by work queued on the previous stream
     cudaStreamSynchronize(dev_->ws_stream);
@@ -169,7 +174,34 @@ Call::Call(const char* name) : name_(name) {
   ok_ = true;
 }
 
+bool Call::capturing() {
+  if (capturing_ < 0) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    capturing_ = 0;
+    if (capturable_) {
+      if (cudaStreamIsCapturing(stream_, &st) != cudaSuccess)
+        cudaGetLastError();  // the legacy stream, while another one is being captured
+      else
+        capturing_ = st != cudaStreamCaptureStatusNone;
+    }
+  }
+  return capturing_ != 0;
+}
+
+bool Call::refuse_host() {
+  if (!capturing()) return false;
+  set_error(kInvalid, "%s: host memory in a call whose stream is being captured", name_);
+  ok_ = false;
+  return true;
+}
+
+void Call::free_graph_memory() {
+  for (void* p : graph_memory_) ACF_CUDA_OK(cudaFreeAsync(p, stream_));
+  graph_memory_.clear();
+}
+
 Call::~Call() {
+  free_graph_memory();
   if (ok_ && !finished_) {
     // early exit after an error: never return while copies still read caller memory
     if (any_host_) cudaStreamSynchronize(stream_);
@@ -178,7 +210,16 @@ Call::~Call() {
 
 void* Call::scratch(size_t bytes) {
   if (!ok_) return nullptr;
-  void* p = dev_->ws.alloc(bytes, stream_);
+  void* p = nullptr;
+  if (capturing()) {
+    if (!ACF_CUDA_OK(cudaMallocAsync(&p, bytes ? bytes : 1, stream_))) {
+      ok_ = false;
+      return nullptr;
+    }
+    graph_memory_.push_back(p);
+    return p;
+  }
+  p = dev_->ws.alloc(bytes, stream_);
   if (!p) {
     set_error(kNoMem, "%s: cannot allocate %zu bytes of device scratch", name_, bytes);
     ok_ = false;
@@ -189,6 +230,7 @@ void* Call::scratch(size_t bytes) {
 const void* Call::in(const void* p, size_t bytes) {
   if (!ok_ || !p) return p;
   if (ptr_kind(p) == PtrKind::Device) return p;
+  if (refuse_host()) return nullptr;
   void* d = scratch(bytes);
   if (!d) return nullptr;
   any_host_ = true;
@@ -202,6 +244,7 @@ const void* Call::in(const void* p, size_t bytes) {
 void* Call::out(void* p, size_t bytes) {
   if (!ok_ || !p) return p;
   if (ptr_kind(p) == PtrKind::Device) return p;
+  if (refuse_host()) return nullptr;
   void* d = scratch(bytes);
   if (!d) return nullptr;
   any_host_ = true;
@@ -212,6 +255,7 @@ void* Call::out(void* p, size_t bytes) {
 void* Call::inout(void* p, size_t bytes) {
   if (!ok_ || !p) return p;
   if (ptr_kind(p) == PtrKind::Device) return p;
+  if (refuse_host()) return nullptr;
   void* d = scratch(bytes);
   if (!d) return nullptr;
   any_host_ = true;
@@ -244,6 +288,7 @@ bool Call::launched(const char* what) {
 bool Call::finish() {
   if (finished_) return ok_;
   finished_ = true;
+  free_graph_memory();  // after the call's kernels in the stream
   if (!ok_) {
     if (any_host_) cudaStreamSynchronize(stream_);
     return false;

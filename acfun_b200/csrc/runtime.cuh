@@ -47,6 +47,7 @@ class Workspace {
   void* alloc(size_t bytes, cudaStream_t s);
   void reset(cudaStream_t s);
   size_t capacity() const { return total_; }
+  bool in_parts() const { return chunks_.size() > 1; }
   void release_all(cudaStream_t s);
 
  private:
@@ -91,7 +92,10 @@ PtrKind ptr_kind(const void* p);
 //   launch(..., c.stream(), c.err()); c.finish();
 class Call {
  public:
-  explicit Call(const char* name);
+  // capturable: the call may be recorded into a graph.  While its stream is being captured it keeps off
+  // the device's workspace, which other calls share and which may move: scratch() is memory that the
+  // graph allocates and frees itself, and host memory is refused.
+  explicit Call(const char* name, bool capturable = false);
   ~Call();
   bool ok() const { return ok_; }
   cudaStream_t stream() const { return stream_; }
@@ -105,6 +109,8 @@ class Call {
   void* inout(void* p, size_t bytes);
   // Plain device scratch for intermediates (256-byte aligned).
   void* scratch(size_t bytes);
+  // A capturable call on a stream that is being captured (looked up when first asked for).
+  bool capturing();
   bool any_host() const { return any_host_; }
   // Record that caller host memory takes part in this call (forces a final synchronise).
   void note_host() { any_host_ = true; }
@@ -131,8 +137,14 @@ class Call {
   DeviceState* dev_ = nullptr;
   std::unique_lock<std::mutex> lock_;
   cudaStream_t stream_ = nullptr;
+  // Resolve a host pointer under capture: an error.
+  bool refuse_host();
+  void free_graph_memory();
   std::vector<Pending> outs_;
+  std::vector<void*> graph_memory_;
   bool ok_ = false, any_host_ = false, finished_ = false;
+  const bool capturable_;
+  int capturing_ = -1;  // not looked up
 };
 
 // Device error word helpers (used by acfun_synchronize and Call::finish).

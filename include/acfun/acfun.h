@@ -173,7 +173,11 @@ int acfun_set_fp32_math(int mode);
  * in the kernels: a bad one skips its sequence (a bad offset those on both sides of it; where offsets
  * decrease, rows of other sequences may be left as they are too) and is reported, as code 1, by the
  * next acfun_synchronize().  Activations and index arrays may be host memory; the cache itself must be
- * device memory. */
+ * device memory.
+ *
+ * Calls on device memory may be recorded into a CUDA graph, once the library has been used on the
+ * device: while the stream set with acfun_set_stream() is being captured, what a call needs besides its
+ * arguments is allocated and freed by the graph, so replays share nothing with other calls. */
 #define ACFUN_F32 0
 #define ACFUN_F16 1
 #define ACFUN_BF16 2
