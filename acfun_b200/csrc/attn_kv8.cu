@@ -10,8 +10,9 @@
 // last of them to finish joins their parts in the order of the chunks, so the result does not
 // depend on who was last.
 //
-// Mathematics.  With q scaled per row by a power of two to fp16 range (exact for what matters:
-// 11 bits below the row's largest element), codes c exact in fp16, S = q.c_k in fp32,
+// Mathematics.  With q scaled per row by a power of two to fp16 range (elements below 2^-14 of the row's
+// largest keep bits down to 2^-24 of it: an absolute error far below that of 11 bits in the largest),
+// codes c exact in fp16, S = q.c_k in fp32,
 //   t = S * (scale * s_k[page]) log2 e + log2 s_v[page],  w = 2^(t - m) in fp16,  O += w c_v,
 //   l += (sum of w over the page's keys, in fp32 before rounding) / s_v[page],  out = O / l.
 // The V scale rides in the exponent, so O needs no per-page scaling and w stays within fp16 range
@@ -28,9 +29,12 @@
 // asynchronously; nothing is shared between warps.
 //
 // Measured (B200): one fp16 token of 64 query heads over 262145 keys of 8 cache heads of 128 elements
-// 101 us, 5.3 TB/s, 81 % of the measured copy rate, at 1.65 GHz under the board's power limit; one
+// 100.6 us, 5.3 TB/s, 81 % of the measured copy rate, at 1.65 GHz under the board's power limit; one
 // token each of 48 sequences of 33 to 16000 keys, 32 query and 8 cache heads, 56 us, 4.0 TB/s, where
-// blocks that find no chunk of their own and the joins of short chunks cost the rest.
+// blocks that find no chunk of their own and the joins of short chunks cost the rest.  16 sequences of
+// 4096 keys with 8 drafted tokens each (32 rows) 56 us where the codes take 20.6; heads of 256, a prompt of
+// 4096 tokens of 16 query and 8 cache heads 986 us.  The keys are divided by max_len, not by the window: one
+// token with a window of 16384 over 262144 keys keeps 32 blocks busy and takes 57 us.
 #include <math.h>
 
 #include <algorithm>
@@ -727,9 +731,11 @@ extern "C" int acfun_kv8_attention(const AcfunKvCache8* cache, const AcfunKvBatc
   // a window that holds any sequence hides nothing (and in the kernels position - window stays in range)
   a.window = window < batch->max_len ? window : 0;
   // Sequences with more than 32 rows per cache head go to the tensor cores' tiles of 128, the others are
-  // streamed.  Measured with 32 query and 8 cache heads of 128 elements, 16 sequences of 4096 keys:
-  // 16 rows 56 us streamed and 88 us tiled, 32 rows 80 and 84, 64 rows 132 and 85.  A batch may hold
-  // both kinds (decode steps beside prompts); where every sequence has max_new tokens it does not.
+  // streamed.  Measured with 32 query and 8 cache heads, 16 sequences of 4096 keys, bf16: heads of 128,
+  // 16 rows 38 us streamed and 71 us tiled, 32 rows 56 and 71, 48 rows 97 and 71, 64 rows 99 and 71;
+  // heads of 64, 39 and 60 at 32 rows, 66 and 60 at 48.  (One sequence of 32768 keys is even at about 20
+  // rows: 16 rows 35 and 46, 32 rows 57 and 49.)  A batch may hold both kinds (decode steps beside
+  // prompts); where every sequence has max_new tokens it does not.
   constexpr long long kStreamRows = 32;
   const long long most = std::min(batch->max_new, tokens) * (long long)a.group;
   const bool tiled = most > kStreamRows && dim != 256;

@@ -24,10 +24,11 @@
 // between its weights and its next scores.
 //
 // Measured (B200, 32 query and 8 cache heads of 128 elements, bf16, causal): a prompt of 8192 tokens
-// 536-548 us, 1.0 PFLOP/s of what the mask leaves, 62 % of the measured bf16 peak, at 1.65 GHz under the
-// board's power limit.  A step of 64 keys of both tiles takes about 1650 cycles; its products need
-// 1280, its 2^x 770 of the special function units (a quarter of them on the FMA units: none 1.22 and
-// half 1.11 times as long per softmax), and it issues 880 instructions per scheduler.  Two threads per
+// 515-536 us, 1.0 PFLOP/s of what the mask leaves, 63 % of the measured bf16 peak, at 1.65 GHz under the
+// board's power limit.  A step of 64 keys of both tiles takes about 1650 cycles; its products need 1280
+// (their arithmetic alone 1024: the operands of S, both from shared memory, 48 cycles of its bandwidth per
+// instruction of 32), its 2^x 770 of the special function units (a quarter of them on the FMA units: none
+// 1.22 and half 1.11 times as long per softmax), and it issues 890 instructions per scheduler.  Two threads per
 // row, with four softmax warps per scheduler instead of two, took 565 us: the exchange of maxima cost
 // more than the latencies it hid.
 // Every wait is bounded (ptx.cuh); on expiry the error word is set and all roles leave.
@@ -58,14 +59,18 @@ constexpr int kKeys = 128;     // keys per stage of K and V
 constexpr int kStep = 64;      // keys of one S product and its softmax
 constexpr int kUnits = kKeys / 16;
 constexpr int kFmaOf4 = 1;      // pairs of four whose 2^x the FMA units compute instead of the special function unit
-constexpr float kLeast = 1e-37f;  // a factor never underflows to 0: a masked score stays -inf under it
+// A factor never underflows to 0: a masked score stays -inf under it.  With q's rows within [2^-40, 2^40] no
+// score that matters has a smaller one.
+constexpr float kLeast = 1e-37f;
 // The offset from which a row's weights are taken from its rounded scores.  The common form, one fused
 // operation on S, sees the rounding of the offset: below this within 2 powers of two, which kTop leaves
 // room for, but from 2^27 on past fp16.
 constexpr float kFar = 0x1p24f;
-// Row tiles from which the key tiles are converted before the kernel (32 query, 8 cache heads of 128:
-// 16 row tiles 34.5 us converted in the kernel and 35.0 us before it, 32 row tiles 60.6 and 55.5), and
-// the most scratch that this may take.
+// Row tiles of a sequence from which the key tiles are converted before the kernel, and the most scratch
+// that this may take.  Measured, one causal bf16 prompt, in the kernel and before it: 32 query and 8 cache
+// heads of 128, 16 row tiles 28.6 and 28.9 us, 24 tiles 37.0 and 37.1, 32 tiles 52.1 and 49.5; 12 and 4
+// heads of 64, 31.4 and 35.1, 43.3 and 43.8, 56.6 and 51.5; 8 and 8 heads of 128, where more blocks wait
+// their turn, 81.5 and 73.9 at 16 tiles already.
 constexpr int kPreRowTiles = 24;
 constexpr size_t kPreBytes = size_t(1) << 30;
 constexpr int kScaleRing = 4;  // the converters are at most two tiles ahead of a softmax

@@ -5,9 +5,10 @@
 // with (a, b) = (i, i + rot/2), or (2i, 2i + 1) when interleaved; elements from rot on are copied.
 // Bound by memory: every element is read and written once.  A block takes a few tokens, computes
 // their cosines and sines once into shared memory (the angle in 64 bits, attn.cuh) and applies
-// them to all heads, 16 bytes per load.  Measured (B200): fp32, 4099 tokens, 20 heads of 64, 42 MB, 9.2 us,
-// 4.6 TB/s, 70 % of the measured copy rate (the input does not come from a cache); one token each of 48
-// sequences, 40 bf16 heads of 128, 8.5 us, which is the host's time for a call.  Requesting the first values
+// them to all heads, 16 bytes per load.  Measured (B200): fp32, 20 heads of 64: 4099 tokens, 42 MB, 9.2 us,
+// 4.6 TB/s, 70 % of the measured copy rate; 65536 tokens, 671 MB, 107 us, 6.3 TB/s, 96 %: the smaller call
+// pays for its start and end.  65536 tokens of 40 bf16 heads of 128 264 us, 5.1 TB/s.  One token each of 48
+// sequences, 40 bf16 heads of 128, 8.6 us, which is the host's time for a call.  Requesting the first values
 // before the cosines and sines took 9.8 us for the former: it costs registers, and other blocks already
 // fill the wait.
 #include <math.h>

@@ -233,7 +233,10 @@ int acfun_rope(const void* x, void* y, int dtype, int tokens, int heads, int dim
  * the sequence first when rope is given (rot a multiple of 16).  The scale of a (page, head) is
  * max(max|x|, 127 * 2^-60) / 127 over the new tokens in the page, code = rint(x * (1 / scale))
  * clamped to +-127.  A page that holds older tokens keeps the larger of its scale and the new
- * one, and when that grows, older codes become rint(code * (old / new)).  Infinities saturate
+ * one, and when that grows, older codes become rint(code * (old / new)).  Within a page the angles are
+ * turned on from token to token in 32 bits, where acfun_rope reduces each in 64: a rotated key is within
+ * 2^-13 of the page's largest element, so a code may differ by a rounding from that of a key which
+ * acfun_rope turned before.  Infinities saturate
  * to +-127 and NaN becomes 0; neither enters a scale.  Pages written must not be shared between
  * sequences. */
 int acfun_kv8_append(const AcfunKvCache8* cache, const AcfunKvBatch* batch, const void* k, const void* v,
