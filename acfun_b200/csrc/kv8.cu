@@ -12,7 +12,7 @@
 // Measured (B200, bf16, 8 heads of 128): append of 65551 tokens with rotation 99 us, 4.1 TB/s of what
 // it has to move, 62 % of the measured copy rate: bound by instructions (18 per value; a page of 128
 // tokens takes a block of 1024 threads, whose barrier per head shows, and whose 64 registers per thread
-// hold for the smaller blocks too: 20 to 44 bytes are spilled, and 208 to 496 with heads of 256).  The same
+// hold for the smaller blocks too: 16 to 44 bytes are spilled, and 208 to 496 with heads of 256).  The same
 // in fp32 145 us (its bytes take 103), with heads of 256 270 us in bf16 (123) and 450 in fp32 (206).  Read of 24 prefixes of 500 to
 // 8191 tokens 84 us, 6.0 TB/s, 92 % of the measured copy rate.
 #include <algorithm>
